@@ -21,6 +21,14 @@ CSRC = HERE / "csrc"
 OBJ = HERE / "build_obj"
 LIB = HERE / "libarbius_kernels.so"
 ARCH = os.environ.get("ARBIUS_ARCH", "gfx950")
+# New sources are compiled without packed fp32 instructions (hipcc forms them from ordinary float code): some of
+# their forms have returned wrong values on gfx950.  The sources below keep them: without, hipcc contracts
+# other mul / add pairs into fmas there, and the models' output bytes, which nodes agree on and
+# tests/golden_cids.json pins, change (21 of its 23 checks).
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+PACKED_FP32 = frozenset((
+    "attention.hip", "attention512.hip", "conv.hip", "convgru.hip", "depthwise.hip", "elementwise.hip",
+    "groupnorm.hip", "h264_intra.hip", "norm.hip", "rvm.hip", "sampler.hip", "temporal_attention.hip"))
 
 
 def _hipcc() -> str:
@@ -38,7 +46,7 @@ def _needs(obj: Path, src: Path) -> bool:
     if not obj.exists():
         return True
     t = obj.stat().st_mtime
-    deps = [src] + list(CSRC.glob("*.h")) + list(CSRC.glob("*.inc"))
+    deps = [src, Path(__file__)] + list(CSRC.glob("*.h")) + list(CSRC.glob("*.inc"))   # this file: the flags
     return any(d.stat().st_mtime > t for d in deps)
 
 
@@ -52,7 +60,8 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False) -> Path:
     def compile_one(src: Path):
         obj = OBJ / (src.stem + ".o")
         if force or _needs(obj, src):
-            cmd = [hipcc, *flags, "-c", str(src), "-o", str(obj)]
+            own = [] if src.name in PACKED_FP32 else NO_PACKED_FP32
+            cmd = [hipcc, *flags, *own, "-c", str(src), "-o", str(obj)]
             if verbose:
                 print(" ".join(cmd), file=sys.stderr)
             r = subprocess.run(cmd, capture_output=True, text=True)
