@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
-from .layers import Embedding, LayerNorm, Linear
+from .layers import Embedding, LayerNorm, Linear, packed_positions
 
 
 @dataclass
@@ -53,11 +53,14 @@ class CLIPLayer(nn.Module):
         self.fc2 = Linear(cfg.mlp, cfg.width)
         self.quick = cfg.quick_gelu
 
-    def forward(self, x):
+    def forward(self, x, documents=None):
         B, N, C = x.shape
         H = self.heads
         qkv = self.ln1.linear(x, self.qkv).view(B, N, 3, H, C // H)   # LayerNorm folded into QKV
-        o = ops.attention(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], causal=True)
+        if documents is None:
+            o = ops.attention(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], causal=True)
+        else:
+            o = ops.masked_attention(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], causal=True, documents=documents)
         x = self.out(o.reshape(B, N, C), residual=x)
         h = self.ln2.linear(x, self.fc1, act="quick_gelu" if self.quick else "gelu")   # LN + act in the GEMM
         return self.fc2(h, residual=x)
@@ -83,3 +86,15 @@ class CLIPTextEncoder(nn.Module):
         eos = ids.argmax(dim=-1)  # EOS has the largest id in the CLIP vocab
         pooled = x[torch.arange(x.shape[0], device=x.device), eos]
         return x, pooled
+
+    def forward_packed(self, ids, offsets):
+        """n prompts of any lengths packed end to end, no padding: ids [T] int64, offsets int32 [n + 1]
+        (prompt t is ids[offsets[t]:offsets[t + 1]], ending with its EOS) -> (hidden [T, width], pooled
+        EOS features [n, width]).  What ``forward`` computes for each prompt alone, up to rounding (the
+        attention walks other key tiles)."""
+        x = self.tok(ids) + self.pos.weight[packed_positions(ids, offsets)[0]]
+        x = x[None]
+        for layer in self.layers[:len(self.layers) - self.cfg.skip_last]:
+            x = layer(x, documents=offsets)
+        x = self.final_ln(x)[0]
+        return x, x[offsets[1:].long() - 1]

@@ -25,6 +25,7 @@ class Linear(nn.Module):
         self.weight = nn.Parameter(torch.empty(cout, cin), requires_grad=False)
         self.bias = nn.Parameter(torch.empty(cout), requires_grad=False) if bias else None
         self.cin, self.cout = cin, cout
+        self.int8 = None              # ops.Int8Rows of the weight: this linear runs in 8 bits (int8_linears)
 
     def reset(self, gen):
         bound = 1.0 / math.sqrt(self.cin)
@@ -33,6 +34,8 @@ class Linear(nn.Module):
             self.bias.data.uniform_(-bound, bound, generator=gen)
 
     def forward(self, x, residual=None, act=None):
+        if self.int8 is not None:
+            return ops.linear_int8(x, self.int8, self.bias, residual=residual, act=act)
         return ops.linear(x, self.weight, self.bias, residual=residual, act=act)
 
     def forward_norm(self, x, norm):
@@ -104,10 +107,15 @@ class LayerNorm(nn.Module):
 
     def linear(self, x, lin: "Linear", residual=None, act=None):
         """act(lin(self(x))) with this LayerNorm (and the activation) folded into the GEMM (ops.ln_linear)."""
+        if lin.int8 is not None:
+            return ops.ln_linear_int8(x, self.weight, self.bias, self.eps, lin.int8, lin.bias, residual=residual,
+                                      act=act)
         return ops.ln_linear(x, self.weight, self.bias, self.eps, lin.weight, lin.bias, residual=residual, act=act)
 
     def linear_geglu(self, x, lin: "Linear"):
         """GEGLU projection of self(x) with this LayerNorm folded in (ops.ln_linear_geglu)."""
+        if lin.int8 is not None:
+            return ops.ln_linear_int8(x, self.weight, self.bias, self.eps, lin.int8, lin.bias, act="geglu")
         return ops.ln_linear_geglu(x, self.weight, self.bias, self.eps, lin.weight, lin.bias)
 
 
@@ -131,6 +139,28 @@ def init_weights(module: nn.Module, seed: int = 0) -> nn.Module:
         if hasattr(m, "reset") and m is not module:
             m.reset(gen)
     return module
+
+
+def packed_positions(ids, offsets):
+    """(position in its prompt, index of its prompt) of every token of prompts packed end to end (offsets
+    int32 [n + 1], the prompts' first tokens and the end)."""
+    at = torch.arange(ids.shape[0], device=ids.device, dtype=torch.int32)
+    doc = torch.searchsorted(offsets, at, right=True) - 1
+    return at - offsets[doc], doc
+
+
+def int8_linears(module: nn.Module, on: bool = True) -> int:
+    """Run the ``Linear`` layers of ``module`` in 8 bits (``ops.linear_int8``; weights quantised here, once, per output
+    channel; activations per token as they come) or, with ``on=False``, in their own type again.  An
+    operator's choice per deployment: other bytes than the 16-bit layers, so never for a registered model
+    whose solutions other nodes verify.  Returns the number of layers.  Call it again after the weights
+    change; linears used through their bare ``weight`` (fused or hoisted projections) stay as they are."""
+    n = 0
+    for m in module.modules():
+        if isinstance(m, Linear):
+            m.int8 = ops.quantize_rows(m.weight) if on else None
+            n += 1
+    return n
 
 
 def timestep_embedding(t, dim, flip_sin_to_cos=True, freq_shift=0.0, max_period=10000):

@@ -22,7 +22,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
-from .layers import Embedding, LayerNorm, Linear
+from .layers import Embedding, LayerNorm, Linear, packed_positions
 
 
 @dataclass
@@ -89,13 +89,16 @@ class XLMRLayer(nn.Module):
         self.fc2 = Linear(cfg.mlp, cfg.width)
         self.ln2 = LayerNorm(cfg.width, cfg.eps)
 
-    def forward(self, x, ns: List[int]):
+    def forward(self, x, ns: List[int], documents=None):
         """x [B, 77, C]; ns[b] = real tokens of sequence b (its keys / values are sliced to them;
-        sequences of equal length share one attention launch)."""
+        sequences of equal length share one attention launch).  ``documents``: x [1, T, C] holds packed
+        sequences at these offsets instead."""
         B, N, C = x.shape
         H = self.heads
         qkv = self.qkv(x).view(B, N, 3, H, C // H)
-        if len(set(ns)) == 1:
+        if documents is not None:
+            o = ops.masked_attention(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], documents=documents)
+        elif len(set(ns)) == 1:
             o = ops.attention(qkv[:, :, 0], qkv[:, :ns[0], 1], qkv[:, :ns[0], 2])
         else:
             o = torch.empty(B, N, H, C // H, dtype=x.dtype, device=x.device)
@@ -139,3 +142,18 @@ class MCLIPText(nn.Module):
             x = layer(x, ns)
         pooled = torch.stack([x[b, :n].float().mean(dim=0) for b, n in enumerate(ns)]).to(x.dtype)
         return x, self.proj(pooled)
+
+    def forward_packed(self, ids, offsets):
+        """n sequences of any lengths packed end to end, no padding: ids [T] int64, offsets int32 [n + 1] ->
+        (full [T, W], pooled [n, proj]): what ``forward`` computes for the real tokens of each sequence,
+        up to rounding."""
+        pos, _ = packed_positions(ids, offsets)
+        x = self.tok(ids) + self.pos(pos + 2) + self.tok_type.weight[0]
+        x = self.ln(x)[None]
+        for layer in self.layers:
+            x = layer(x, None, documents=offsets)
+        x = x[0]
+        off = offsets.long()
+        total = torch.nn.functional.pad(x.double().cumsum(dim=0), (0, 0, 1, 0))[off]     # fixed order, no atomics
+        pooled = (total[1:] - total[:-1]) / (off[1:] - off[:-1])[:, None]
+        return x, self.proj(pooled.to(x.dtype))

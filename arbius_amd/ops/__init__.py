@@ -304,6 +304,123 @@ def ln_linear_geglu(x, gamma, beta, eps, w, b=None):
     return linear_geglu(layer_norm(x, gamma, beta, eps), w, b)
 
 
+# --------------------------------------------------------------------------- 8-bit linears
+INT8_MAX_K = 133000          # 127^2 K stays below 2^31: the integer sums never wrap
+
+
+class Int8Rows:
+    """Rows of K values in 8 bits: value = q * scale, ``q`` int8 [R, K] and ``scale`` fp32 [R] (one per row: per
+    token of an activation, per output channel of a weight).  Built by ``quantize_rows`` /
+    ``ln_quantize_rows``, or around tensors a program already holds: rows on 16-byte boundaries (stride
+    and base multiples of 16, the row padded up to one), never copied.  ``shape`` / ``dtype``: of the
+    tensor the rows stand for."""
+    __slots__ = ("q", "scale", "shape", "dtype", "zero_tail")
+
+    def __init__(self, q, scale, shape=None, dtype=torch.bfloat16):
+        if q.dtype != torch.int8 or scale.dtype != torch.float32 or q.device != scale.device:
+            raise TypeError("Int8Rows: q int8 and scale fp32 on one device")
+        if q.dim() != 2 or tuple(scale.shape) != (q.shape[0],) or not scale.is_contiguous():
+            raise ValueError(f"Int8Rows: q {tuple(q.shape)} scale {tuple(scale.shape)} (q [R, K], scale [R])")
+        R, K = q.shape
+        shape = (R, K) if shape is None else tuple(shape)
+        if not 1 <= K <= INT8_MAX_K or shape[-1] != K or math.prod(shape[:-1]) != R:
+            raise ValueError(f"Int8Rows: q {tuple(q.shape)} for shape {shape} (1 <= K <= {INT8_MAX_K})")
+        pad = -(-K // 16) * 16
+        if q.stride(1) != 1 or (R and (q.data_ptr() % 16 or q.stride(0) % 16 or q.stride(0) < pad)):
+            raise ValueError(f"Int8Rows: rows need stride >= {pad} and, like the base, a multiple of 16 bytes")
+        if R and q.storage_offset() + (R - 1) * q.stride(0) + pad > q.untyped_storage().nbytes():
+            raise ValueError("Int8Rows: the storage ends inside the last row's padding")
+        self.q, self.scale, self.shape, self.dtype = q, scale, shape, dtype
+        self.zero_tail = pad == K
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def dequantize(self):
+        return (self.q.float() * self.scale[:, None]).to(self.dtype).reshape(self.shape)
+
+
+def _quantize(x, norm, op):
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= INT8_MAX_K:
+        raise ValueError(f"{op}: x {tuple(x.shape)} (a last dim of 1 .. {INT8_MAX_K} expected)")
+    if not x.is_floating_point():
+        raise TypeError(f"{op}: got {x.dtype}")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError(f"{op}: inference only (no gradients)")
+    if _hip(x):
+        q, scale = _lib.quantize_rows(x, norm)
+    else:
+        if norm is not None:
+            x32 = F.layer_norm(x.float(), (x.shape[-1],), norm[0].float(), norm[1].float(), norm[2])
+        q, scale = ref.quantize_rows(x if norm is None else x32)
+        pad = -q.shape[1] % 16
+        if pad:
+            q = F.pad(q, (0, pad))[:, :x.shape[-1]]
+    rows = Int8Rows(q, scale, x.shape, x.dtype)
+    rows.zero_tail = True
+    return rows
+
+
+def quantize_rows(x):
+    """x [..., K] as ``Int8Rows``: scale = max|row| / 127, q = round(127 x / max|row|) (half to even, the correctly
+    rounded quotient).  A zero row gets scale 0; a row that holds a NaN or an infinity gets scale NaN,
+    so every product with it is NaN.  GPU: bf16 / fp16, one HIP pass."""
+    return _quantize(x, None, "quantize_rows")
+
+
+def ln_quantize_rows(x, gamma, beta, eps):
+    """``quantize_rows`` of LayerNorm(x), the normalised row held in fp32 until it is quantised."""
+    for t in (gamma, beta):
+        if tuple(t.shape) != (x.shape[-1],) or t.dtype != x.dtype or t.device != x.device or not t.is_contiguous():
+            raise ValueError(f"ln_quantize_rows: gamma / beta must be contiguous {x.dtype} [{x.shape[-1]}]")
+    return _quantize(x, (gamma, beta, float(eps)), "ln_quantize_rows")
+
+
+def linear_int8(x, w, b=None, residual=None, act=None):
+    """y = act(x @ w^T + b (+ residual)) with both operands in 8 bits: x [..., K] is quantised row by row
+    (``quantize_rows``; an ``Int8Rows`` is taken as it is, to share one quantisation between linears), w is
+    the ``Int8Rows`` [N, K] of the weight.  act None / "gelu" / "quick_gelu" as in ``linear``, or "geglu":
+    w, b = [value | gate] rows, y [..., N / 2] = value * gelu(gate) (no residual).
+
+    The integer sums are exact, so y does not depend on tiles, splits or the other rows of the batch.
+    GPU: b, residual and y in x's dtype (bf16 / fp16) (csrc/linear_int8.hip).  Inference only."""
+    if not isinstance(w, Int8Rows) or len(w.shape) != 2:
+        raise TypeError("linear_int8: w must be the Int8Rows of a weight [N, K]")
+    if not isinstance(x, (torch.Tensor, Int8Rows)):
+        raise TypeError(f"linear_int8: x is a {type(x).__name__}")
+    N, K = w.shape
+    if x.shape[-1] != K or x.device != w.device:
+        raise ValueError(f"linear_int8: x {tuple(x.shape)} on {x.device}, w {w.shape} on {w.device}")
+    if act not in _lib._INT8_ACT:
+        raise ValueError(f"linear_int8: act {act!r}")
+    if act == "geglu" and (N % 2 or residual is not None):
+        raise ValueError("linear_int8: geglu needs an even number of weight rows and takes no residual")
+    shape = tuple(x.shape[:-1])
+    for name, t, want in (("b", b, (N,)), ("residual", residual, shape + (N,))):
+        if t is None:
+            continue
+        if tuple(t.shape) != want or t.dtype != x.dtype or t.device != w.device:
+            raise ValueError(f"linear_int8: {name} {tuple(t.shape)} {t.dtype}, {want} {x.dtype} expected")
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError("linear_int8: inference only (no gradients)")
+    b = None if b is None else b.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    rows = x if isinstance(x, Int8Rows) else quantize_rows(x)
+    q = rows.q
+    if not rows.zero_tail:               # the caller's own rows: what follows column K must not reach the sums
+        q = F.pad(q, (0, -K % 16))[:, :K]
+    impl = _lib if _hip(w.q) else ref
+    if impl is _lib and rows.dtype not in _lib._EL:
+        raise TypeError(f"linear_int8: the HIP kernel writes bf16 or fp16, not {rows.dtype}")
+    return impl.linear_int8(q, rows.scale, w.q, w.scale, b, residual, act, shape, rows.dtype)
+
+
+def ln_linear_int8(x, gamma, beta, eps, w, b=None, residual=None, act=None):
+    """``linear_int8`` of LayerNorm(x): normalised and quantised in one pass over x."""
+    return linear_int8(ln_quantize_rows(x, gamma, beta, eps), w, b, residual, act)
+
+
 class CatPair:
     """The channel concat [a | b] of two channels-last tensors, NOT materialised: the UNet up-path
     skip connection.  Its consumers (GroupNorm statistics, the GroupNorm table-apply pass and the
@@ -636,6 +753,76 @@ def temporal_attention(q, k, v, scale=None):
 
 
 TEMPORAL_MAX_FRAMES = 96     # csrc/temporal_attention.hip keeps <= 96 frames in registers
+
+
+def _index_arg(name, t, like, shapes):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != like.device:
+        raise TypeError(f"masked_attention: {name} must be an int32 tensor on {like.device}")
+    if tuple(t.shape) not in shapes or (t.dim() and t.stride(-1) != 1):
+        raise ValueError(f"masked_attention: {name} has shape {tuple(t.shape)} (contiguous {shapes} expected)")
+
+
+def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=None, prefix=None, documents=None,
+                     softcap=None, slopes=None):
+    """Attention with masks and score transforms: q [B, Nq, H, D], k / v [B, Nk, Hkv, D] (last dim contiguous,
+    H a multiple of Hkv: query head h reads key / value head h // (H // Hkv)) -> [B, Nq, H, D].
+
+        s_ij = cap tanh(scale q_i.k_j / cap) - slopes[h] |p_i - j|,  o_i = sum_j softmax_j(s_ij) v_j
+
+    over the keys every given mask leaves; a query they leave none gets zeros, and what masked keys and
+    values hold (NaN, infinities, memory never written) does not matter.  p_i = q_start + i is the
+    position of query i among the keys.  All optional:
+
+    * ``causal``: keys j <= p_i; with ``prefix`` also the first ``prefix`` keys (of the document, if any)
+    * ``q_start``: position of the first query (an int, or int32 [B]; default 0): new tokens of a sequence
+      whose earlier keys are cached
+    * ``lengths`` int32 [B]: keys j < lengths[b]
+    * ``documents`` int32 [n + 1] (or [B, n + 1]): offsets of n documents packed end to end; a query sees
+      only keys of the document that holds its position (outside of all: nothing)
+    * ``prefix`` int32 [B], or with ``documents`` [n] (or [B, n]): needs ``causal``
+    * ``softcap``: cap of the scores;  ``slopes`` fp32 [H]: linear bias by distance
+
+    GPU: bf16 / fp16, D % 8 == 0, D <= 256 (csrc/masked_attention.hip).  Inference only."""
+    if q.dim() != 4 or k.dim() != 4 or tuple(k.shape) != tuple(v.shape):
+        raise ValueError(f"masked_attention: q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
+    B, Nq, H, D = q.shape
+    if k.shape[0] != B or k.shape[3] != D or k.shape[2] < 1 or H % k.shape[2] or D < 1:
+        raise ValueError(f"masked_attention: q {tuple(q.shape)} does not go with k / v {tuple(k.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise TypeError("masked_attention: q, k and v must share dtype and device")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise RuntimeError("masked_attention: inference only (no gradients)")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"masked_attention: scale {scale}")
+    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
+        raise ValueError(f"masked_attention: softcap {softcap} (a positive number expected)")
+    if isinstance(q_start, torch.Tensor):
+        _index_arg("q_start", q_start, q, [(B,)])
+    else:
+        q_start = 0 if q_start is None else int(q_start)
+        if not 0 <= q_start < 2 ** 31 - Nq:
+            raise ValueError(f"masked_attention: q_start {q_start}")
+    if lengths is not None:
+        _index_arg("lengths", lengths, q, [(B,)])
+    n = 0
+    if documents is not None:
+        n = documents.shape[-1] - 1 if isinstance(documents, torch.Tensor) and documents.dim() else 0
+        if n < 1:
+            raise ValueError("masked_attention: documents needs the offsets of one document at least")
+        _index_arg("documents", documents, q, [(n + 1,), (B, n + 1)])
+    if prefix is not None:
+        if not causal:
+            raise ValueError("masked_attention: prefix needs causal=True")
+        _index_arg("prefix", prefix, q, [(B,)] if documents is None else [(n,), (B, n)])
+    if slopes is not None and (not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32
+                               or slopes.device != q.device or tuple(slopes.shape) != (H,)
+                               or not slopes.is_contiguous()):
+        raise ValueError(f"masked_attention: slopes must be contiguous fp32 [{H}] on {q.device}")
+    if Nq >= 2 ** 31 or k.shape[1] >= 2 ** 31:
+        raise ValueError("masked_attention: more than 2^31 - 1 queries or keys")
+    impl = _lib if _hip(q) else ref
+    return impl.masked_attention(q, k, v, scale, bool(causal), q_start, lengths, prefix, documents, softcap, slopes)
 
 
 # --------------------------------------------------------------------------- ConvGRU

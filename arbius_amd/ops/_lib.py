@@ -90,6 +90,11 @@ _SIGS = {
                                                                     c_void_p]),
     "arb_h264_intra_host": (c_int, [c_void_p] * 3 + [c_int] * 4 + [c_void_p, ctypes.c_longlong, c_void_p, c_void_p]),
     "arb_set_h264_sync": (None, [c_int]),
+    "arb_quantize_rows": (c_int, [c_void_p, c_long, c_void_p, c_void_p, c_float, c_void_p, c_int, c_void_p, c_long,
+                                  c_int, c_int, c_void_p]),
+    "arb_linear_int8": (c_int, [c_void_p, c_long, c_void_p, c_void_p, c_long] + [c_void_p] * 4 + [c_int] * 5
+                        + [c_void_p]),
+    "arb_masked_attention": (c_int, [c_void_p] * 11 + [c_float, c_float, c_int, c_void_p]),
 }
 
 
@@ -1098,3 +1103,102 @@ def h264_intra_host(y, cb, cr, qp: int, return_ws: bool = False):
         raise RuntimeError(f"h264_intra_host failed ({rc})")
     return (out, meta, ws) if return_ws else (out, meta)
 
+
+# --------------------------------------------------------------------------- 8-bit linears, masked attention
+_EL = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _el(op, t):
+    try:
+        return _EL[t.dtype]
+    except KeyError:
+        raise TypeError(f"{op}: the HIP kernel takes bf16 or fp16 tensors, got {t.dtype}") from None
+
+
+class _on:
+    """Launch on ``t``'s device and its current stream, whatever the caller's current device is."""
+    __slots__ = ("guard",)
+
+    def __init__(self, t):
+        dev = t.device
+        same = _AUDIT is not None or dev.index is None or dev.index == torch.cuda.current_device()
+        self.guard = None if same else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return _stream()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _rows2d(x):
+    """x [..., K] as rows [R, K] with one row stride (a copy only where the leading dims do not collapse)."""
+    if x.dim() == 2 and x.stride(1) == 1:
+        return x
+    x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
+def quantize_rows(x, norm=None):
+    """x [..., K] -> (q int8 [R, K] on rows of a multiple of 16 bytes whose tails are zero, scale fp32 [R]);
+    norm = (gamma, beta, eps): of LayerNorm(x) (csrc/linear_int8.hip)."""
+    el = _el("quantize_rows", x)
+    K = x.shape[-1]
+    x2 = _rows2d(x)
+    R, ldq = x2.shape[0], -(-K // 16) * 16
+    q = torch.empty(R, ldq, dtype=torch.int8, device=x.device)
+    scale = torch.empty(R, dtype=torch.float32, device=x.device)
+    gamma, beta, eps = norm if norm is not None else (None, None, 0.0)
+    if R:
+        with _on(x) as stream:
+            _check(_fn("arb_quantize_rows")(_p(x2), x2.stride(0), _p(gamma), _p(beta), float(eps), _p(q), ldq,
+                                            _p(scale), R, K, el, stream), "quantize_rows")
+    return (q if ldq == K else q[:, :K]), scale
+
+
+_INT8_ACT = {None: 0, "gelu": 1, "quick_gelu": 2, "geglu": 3}
+
+
+def linear_int8(q, sx, w, sw, b, residual, act, shape, dtype):
+    """q [M, K] / w [N, K] int8 rows with fp32 scales -> act(sx sw (q . w) + b + residual) [*shape, N]."""
+    el = _EL[dtype]
+    M, K = q.shape
+    N = w.shape[0]
+    y = torch.empty(*shape, N // 2 if act == "geglu" else N, dtype=dtype, device=q.device)
+    audit_note("linear_int8", M=M, N=N, K=K)
+    if y.numel():
+        with _on(q) as stream:
+            _check(_fn("arb_linear_int8")(_p(q), q.stride(0), _p(sx), _p(w), w.stride(0), _p(sw), _p(b), _p(residual),
+                                          _p(y), M, N, K, _INT8_ACT[act], el, stream), "linear_int8")
+    return y
+
+
+def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents, softcap, slopes):
+    """Arguments as checked by ``ops.masked_attention`` (csrc/masked_attention.hip)."""
+    el = _el("masked_attention", q)
+    B, Nq, H, D = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    if D % 8 or D > 256:
+        raise ValueError(f"masked_attention: D={D} not a multiple of 8 up to 256")
+    for t in (q, k, v):
+        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+            raise ValueError("masked_attention: last dim must be contiguous, strides/base 16B aligned")
+    o = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
+    if not o.numel():
+        return o
+    if not Nk:
+        return o.zero_()
+    starts = isinstance(q_start, torch.Tensor)
+    docs_sb = documents.stride(0) if documents is not None and documents.dim() == 2 else 0
+    prefix_sb = 0 if prefix is None else prefix.stride(0) if documents is None or prefix.dim() == 2 else 0
+    strides = (c_long * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
+    ints = (c_long * 11)(B, H, Hkv, Nq, Nk, D, int(causal), 0 if starts else q_start,
+                         0 if documents is None else documents.shape[-1] - 1, docs_sb, prefix_sb)
+    with _on(q) as stream:
+        _check(_fn("arb_masked_attention")(_p(q), _p(k), _p(v), _p(o), strides, ints, _p(q_start if starts else None),
+                                           _p(lengths), _p(documents), _p(prefix), _p(slopes), float(scale),
+                                           float(softcap or 0.0), el, stream), "masked_attention")
+    return o

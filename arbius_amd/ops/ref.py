@@ -99,6 +99,96 @@ def attention(q, k, v, scale=None, causal=False):
     return o.transpose(1, 2).to(q.dtype)
 
 
+def quantize_rows(x):
+    """x [..., K] -> (q int8 [R, K], scale fp32 [R]): scale = max|row| / 127, q = round(127 x / max|row|), half
+    to even (in 64 bits: the correctly rounded quotient); a zero row gets scale 0, a row with a NaN or an
+    infinity scale NaN, both q = 0."""
+    x = x.reshape(-1, x.shape[-1]).float()
+    a = x.abs().amax(dim=1)
+    scale = torch.where(a.isfinite(), a / 127.0, torch.full_like(a, float("nan")))
+    q = torch.round(x.double() * 127.0 / a.double()[:, None])
+    q = torch.where((a > 0)[:, None] & a.isfinite()[:, None], q, torch.zeros_like(q))
+    return q.to(torch.int8), scale
+
+
+def linear_int8(q, sx, w, sw, b, residual, act, shape, dtype):
+    """act(sx sw (q . w) + b + residual) in fp32 over the exact integer sums, rounded once to ``dtype``."""
+    y = (q.double() @ w.double().t()).float() * sx[:, None] * sw
+    if b is not None:
+        y = y + b.float()
+    if residual is not None:
+        y = y + residual.float().reshape(y.shape)
+    if act == "gelu":
+        y = F.gelu(y)
+    elif act == "quick_gelu":
+        y = y * torch.sigmoid(1.702 * y)
+    elif act == "geglu":
+        a, gate = y.chunk(2, dim=-1)
+        y = a * F.gelu(gate)
+    return y.to(dtype).reshape(*shape, y.shape[-1])
+
+
+def key_runs(Nq, Nk, B, causal, q_start, lengths, prefix, documents, device):
+    """(lo, hi) [B, Nq]: the run of keys each query of ``masked_attention`` sees, and the positions."""
+    start = q_start.long() if isinstance(q_start, torch.Tensor) else torch.full((B,), int(q_start), device=device)
+    p = start.to(device)[:, None] + torch.arange(Nq, device=device)
+    lo, hi = torch.zeros_like(p), torch.full_like(p, Nk)
+    doc = torch.zeros_like(p)
+    if documents is not None:
+        off = documents.long().reshape(-1, documents.shape[-1]).expand(B, -1).contiguous()
+        doc = torch.searchsorted(off, p.contiguous(), right=True) - 1
+        inside = (doc >= 0) & (doc < off.shape[1] - 1)
+        doc = doc.clamp(0, off.shape[1] - 2)
+        lo = off.gather(1, doc).clamp(0, Nk)
+        hi = torch.where(inside, off.gather(1, doc + 1).clamp(max=Nk), torch.zeros_like(hi))
+    if causal:
+        seen = p + 1
+        if prefix is not None:
+            shown = prefix.long()
+            if documents is None:
+                shown = shown.reshape(B, 1).expand_as(p)
+            else:
+                shown = shown.reshape(-1, shown.shape[-1]).expand(B, -1).gather(1, doc)
+            seen = torch.maximum(seen, lo + shown)
+        hi = torch.minimum(hi, seen)
+    if lengths is not None:
+        hi = torch.minimum(hi, lengths.long()[:, None])
+    return lo, hi, p
+
+
+def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents, softcap, slopes):
+    """q [B, Nq, H, D], k / v [B, Nk, Hkv, D] -> [B, Nq, H, D]; see ``ops.masked_attention``."""
+    B, Nq, H, _ = q.shape
+    Nk, group = k.shape[1], H // k.shape[2]
+    if Nk == 0:
+        return torch.zeros_like(q)
+    lo, hi, p = key_runs(Nq, Nk, B, causal, q_start, lengths, prefix, documents, q.device)
+    j = torch.arange(Nk, device=q.device)
+    ok = ((j >= lo[..., None]) & (j < hi[..., None]))[:, None]                      # [B, 1, Nq, Nk]
+    qf = q.float().transpose(1, 2)
+    kf, vf = (t.float().transpose(1, 2).repeat_interleave(group, dim=1) for t in (k, v))
+    s = torch.matmul(qf, kf.transpose(-1, -2)) * scale
+    if softcap:
+        s = softcap * torch.tanh(s / softcap)
+    if slopes is not None:
+        s = s - slopes.float()[None, :, None, None] * (p[..., None] - j).abs().float()[:, None]
+    s = torch.where(ok, s, torch.full_like(s, float("-inf")))
+    m = s.amax(dim=-1, keepdim=True)
+    e = torch.exp(s - torch.where(m == float("-inf"), torch.zeros_like(m), m))
+    total = e.sum(dim=-1, keepdim=True)
+    w = torch.where(total == 0, torch.zeros_like(e), e / total)         # no key (or none but scores of -inf): zeros
+    # a masked value never reaches the sum, whatever it holds (0 * NaN would)
+    fine = torch.isfinite(vf)
+    o = torch.matmul(w, torch.where(fine, vf, torch.zeros_like(vf)))
+    if not bool(fine.all()):
+        seen = ok.to(w.dtype).expand(B, H, Nq, Nk)
+        for bad, val in ((vf.isnan(), float("nan")), (vf == float("inf"), float("inf")),
+                         (vf == -float("inf"), -float("inf"))):
+            o = o + torch.where(torch.matmul(seen, bad.to(w.dtype)) > 0, torch.full_like(o, val),
+                                torch.zeros_like(o))
+    return o.transpose(1, 2).to(q.dtype)
+
+
 def geglu(h):
     """h [..., 2F] -> a * gelu(gate) with (a, gate) = split(h)."""
     a, gate = h.float().chunk(2, dim=-1)

@@ -1,0 +1,343 @@
+"""8-bit linears (``ops.quantize_rows`` / ``ln_quantize_rows`` / ``linear_int8`` / ``ln_linear_int8``) against their
+definitions in 64 bits, on the CPU reference and on the HIP kernels.
+
+Tolerances.  quantize_rows: none (q is the correctly rounded quotient, scale one fp32 division).
+linear_int8: the integer sum is exact; its conversion to fp32, two scale products and up to two additions round
+5 times at 2^-24 of the largest magnitude, the activation adds at most 4e-7 of it (GELU: 1.5e-7 on erf, raw
+exp2 / rcp 2^-22): 2^-20 of the magnitude covers both.  Then one rounding to the output type: half a step,
+``finfo.eps / 2`` of the value (2^-25 in fp16's subnormals).
+ln_quantize_rows: the fp32 LayerNorm is within 2^-17 of the row's largest value (two block sums of at most 2048
+terms and five roundings), so q is within half a step plus 127 * 2^-17 of the 64-bit quotient."""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from arbius_amd import ops
+from arbius_amd.models import layers
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(*shape, seed=0, dtype=torch.float32, device="cpu"):
+    return torch.randn(*shape, generator=gen(seed)).to(dtype).to(device)
+
+
+def quantize64(x):
+    x = x.double()
+    a = x.abs().amax(dim=-1, keepdim=True)
+    q = torch.where(a > 0, torch.round(x * 127.0 / a), torch.zeros_like(x))
+    return q, (a / 127.0)
+
+
+def gelu64(x):
+    return 0.5 * x * torch.special.erfc(-x / math.sqrt(2.0))
+
+
+def linear64(q, sx, wq, sw, b, r, act):
+    t = (q.double() @ wq.double().t()) * sx.double().reshape(-1, 1) * sw.double()
+    y, mag = t, t.abs()
+    for term in (b, r):
+        if term is not None:
+            y, mag = y + term.double(), mag + term.double().abs()
+    if act == "gelu":
+        y = gelu64(y)
+    elif act == "quick_gelu":
+        y = y * torch.sigmoid(1.702 * y)
+    elif act == "geglu":
+        h = y.shape[-1] // 2
+        y, mag = y[:, :h] * gelu64(y[:, h:]), mag[:, :h] * mag[:, h:]
+    return y, mag
+
+
+def check(y, want, mag):
+    half = torch.finfo(y.dtype).eps / 2
+    err = (y.cpu().double().reshape(want.shape) - want).abs()
+    over = err - (half * want.abs() + 2.0 ** -20 * mag + 2.0 ** -25)
+    assert bool((over <= 0).all()), f"over the bound by {over.max().item():.3g}"
+
+
+def rows(n, k, seed, device, dtype=torch.bfloat16):
+    return ops.quantize_rows(randn(n, k, seed=seed, dtype=dtype, device=device) * (0.5 / math.sqrt(k)))
+
+
+# ------------------------------------------------------------------ quantize_rows
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 16), (5, 77), (4, 320), (2, 2048), (7, 1101), (1, 20000), (300, 48)])
+def test_quantize_rows_is_the_rounded_quotient(device, dtype, m, k):
+    x = randn(m, k, seed=k, dtype=DTYPES[dtype], device=device)
+    r = ops.quantize_rows(x)
+    q, _ = quantize64(x.cpu())
+    assert r.q.dtype == torch.int8 and torch.equal(r.q.cpu().double(), q)
+    assert torch.equal(r.scale.cpu(), x.cpu().float().abs().amax(dim=1) / 127.0)
+    assert r.shape == (m, k) and r.dtype == x.dtype
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_rows_half_steps_go_to_even(device, dtype):
+    """Every row holds a = 127 * 2^e and the exact half steps (k + 1/2) 2^e and their neighbours."""
+    dt = DTYPES[dtype]
+    out = []
+    for e in (0, -6, 5):
+        v = torch.arange(-126, 127, dtype=torch.float64) + 0.5
+        x = torch.cat([torch.tensor([127.0], dtype=torch.float64), v]) * 2.0 ** e
+        out.append(x[:254])
+    x = torch.stack(out).to(dt)
+    x = torch.cat([x, torch.nextafter(x.float(), torch.full_like(x.float(), 1e9)).to(dt)])
+    x[3:, 0] = x[:3, 0]
+    r = ops.quantize_rows(x.to(device))
+    q, _ = quantize64(x)
+    assert torch.equal(r.q.cpu().double(), q)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_quantize_rows_extremes(device):
+    big, tiny = torch.finfo(torch.bfloat16).max, 2.0 ** -130
+    x = torch.zeros(7, 40)
+    x[1] = torch.linspace(-1, 1, 40) * big
+    x[2] = torch.linspace(-1, 1, 40) * tiny
+    x[3, 5], x[4, 6], x[5, 39] = float("nan"), float("inf"), -float("inf")
+    x[3:6, :4] = 1.0
+    x[6, 7] = -2.0
+    x = x.to(torch.bfloat16)
+    r = ops.quantize_rows(x.to(device))
+    q, _ = quantize64(x[[0, 1, 2, 6]])
+    assert torch.equal(r.q.cpu()[[0, 1, 2, 6]].double(), q)
+    assert r.scale[0] == 0 and r.scale.cpu()[3:6].isnan().all() and not bool(r.q[3:6].any())
+    # what such a row yields: zeros (+ bias) and NaN
+    w = rows(24, 40, 1, device)
+    y = ops.linear_int8(x.to(device), w)
+    assert not bool(y[0].any()) and bool(y[3:6].isnan().all()) and bool(y[[2, 6]].isfinite().all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_quantize_rows_strided_views(device):
+    base = randn(3, 5, 4, 96, seed=2, dtype=torch.bfloat16, device=device)
+    for x in (base[:, :, 1], base[:, 2], base[1, :, :, 8:72], base[..., 3:80], base.transpose(0, 1), base[..., ::2],
+              base[:1, :1, :1].expand(4, 1, 1, 96)):
+        a, b = ops.quantize_rows(x), ops.quantize_rows(x.clone(memory_format=torch.contiguous_format))
+        assert a.shape == tuple(x.shape) and torch.equal(a.q, b.q) and torch.equal(a.scale, b.scale)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k", [(1, 8), (5, 77), (3, 320), (4, 768), (2, 2048), (6, 1001), (130, 64)])
+def test_ln_quantize_rows(device, dtype, m, k):
+    dt = DTYPES[dtype]
+    x = (randn(m, k, seed=3) * 3 + 0.5).to(dt)
+    gamma, beta = (1 + 0.2 * randn(k, seed=4)).to(dt), (0.2 * randn(k, seed=5)).to(dt)
+    r = ops.ln_quantize_rows(x.to(device), gamma.to(device), beta.to(device), 1e-5)
+    x64 = x.double()
+    y = (x64 - x64.mean(1, keepdim=True)) / torch.sqrt(x64.var(1, unbiased=False, keepdim=True) + 1e-5)
+    y = y * gamma.double() + beta.double()
+    a = y.abs().amax(dim=1, keepdim=True)
+    assert bool(((r.scale.cpu().double()[:, None] * 127 / a - 1).abs() <= 2.0 ** -16).all())
+    assert bool(((r.q.cpu().double() - 127 * y / a).abs() <= 0.5 + 127 * 2.0 ** -17).all())
+
+
+# ------------------------------------------------------------------ linear_int8
+SHAPES = [(1, 64, 64), (1, 16, 1), (1, 2048, 520), (2, 100, 30), (7, 1101, 33), (16, 640, 256), (17, 4096, 96),
+          (33, 130, 257), (64, 128, 512), (100, 320, 960), (129, 1000, 200), (257, 768, 384), (300, 256, 1030),
+          (513, 48, 130)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_linear_int8_shapes(device, dtype, m, k, n):
+    dt = DTYPES[dtype]
+    x, w = randn(m, k, seed=m, dtype=dt, device=device), rows(n, k, n, device, dt)
+    b, r = randn(n, seed=1, dtype=dt, device=device), randn(m, n, seed=2, dtype=dt, device=device)
+    qx = ops.quantize_rows(x)
+    for bias, res in ((None, None), (b, None), (b, r)):
+        y = ops.linear_int8(x, w, bias, residual=res)
+        assert y.dtype == dt and tuple(y.shape) == (m, n)
+        cpu = [None if t is None else t.cpu() for t in (bias, res)]
+        check(y, *linear64(qx.q.cpu(), qx.scale.cpu(), w.q.cpu(), w.scale.cpu(), *cpu, None))
+    assert torch.equal(ops.linear_int8(qx, w, b, residual=r), ops.linear_int8(x, w, b, residual=r))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["gelu", "quick_gelu", "geglu"])
+@pytest.mark.parametrize("m,k,n", [(1, 256, 512), (5, 77, 34), (40, 320, 640), (200, 128, 1034), (300, 640, 512)])
+def test_linear_int8_activations(device, dtype, act, m, k, n):
+    dt = DTYPES[dtype]
+    x, w = (2 * randn(m, k, seed=m)).to(dt).to(device), ops.quantize_rows(
+        randn(n, k, seed=n, dtype=dt, device=device) / math.sqrt(k))
+    b = randn(n, seed=1, dtype=dt, device=device)
+    qx = ops.quantize_rows(x)
+    y = ops.linear_int8(x, w, b, act=act)
+    check(y, *linear64(qx.q.cpu(), qx.scale.cpu(), w.q.cpu(), w.scale.cpu(), b.cpu(), None, act))
+    if act != "geglu":
+        r = randn(m, n, seed=2, dtype=dt, device=device)
+        check(ops.linear_int8(x, w, b, residual=r, act=act),
+              *linear64(qx.q.cpu(), qx.scale.cpu(), w.q.cpu(), w.scale.cpu(), b.cpu(), r.cpu(), act))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_int8_full_scale_sums(device):
+    """Every product 127 * 127 of one sign: the largest sums, exact to the last bit before the scales."""
+    for k in (16, 1000, 9001, 133000):
+        q = torch.full((3, k), 127, dtype=torch.int8)
+        q[1] = -127
+        q[2, 0] = 126
+        pad = -k % 16
+        store = torch.nn.functional.pad(q, (0, pad)).to(device)
+        x = ops.Int8Rows(store[:, :k], torch.ones(3, device=device), dtype=torch.bfloat16)
+        y = ops.linear_int8(x, x)
+        want = (q.double() @ q.double().t()).float().to(torch.bfloat16)
+        assert torch.equal(y.cpu(), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_int8_rows_with_anything_behind_them(device):
+    """Rows cut out of a wider int8 buffer: neither the buffer's other columns nor its rows get in."""
+    k, wide = 37, 96
+    bx = torch.randint(-127, 128, (9, wide), generator=gen(1), dtype=torch.int8).to(device)
+    bw = torch.randint(-127, 128, (21, wide), generator=gen(2), dtype=torch.int8).to(device)
+    sx, sw = torch.rand(9, generator=gen(3)).to(device), torch.rand(21, generator=gen(4)).to(device)
+    x, w = ops.Int8Rows(bx[:, 16:16 + k], sx, (3, 3, k), torch.float16), ops.Int8Rows(bw[:, 48:48 + k], sw)
+    y = ops.linear_int8(x, w)
+    assert tuple(y.shape) == (3, 3, 21)
+    want, mag = linear64(x.q.cpu(), sx.cpu(), w.q.cpu(), sw.cpu(), None, None, None)
+    check(y.reshape(9, 21) * 2.0 ** -8, want * 2.0 ** -8, mag)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_int8_batch_invariance_and_leading_dims(device):
+    x = randn(6, 31, 200, seed=7, dtype=torch.bfloat16, device=device)
+    w, b = rows(136, 200, 8, device), randn(136, seed=9, dtype=torch.bfloat16, device=device)
+    y = ops.linear_int8(x, w, b, act="gelu")
+    assert tuple(y.shape) == (6, 31, 136)
+    for i in range(6):
+        assert torch.equal(ops.linear_int8(x[i], w, b, act="gelu"), y[i])
+    assert torch.equal(ops.linear_int8(x[2, 5:6], w, b, act="gelu")[0], y[2, 5])
+    assert tuple(ops.linear_int8(x[0, 0], w).shape) == (136,)
+    assert tuple(ops.linear_int8(x[:0], w).shape) == (0, 31, 136)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_ln_linear_int8_is_its_two_halves(device):
+    x = randn(50, 320, seed=1, dtype=torch.bfloat16, device=device)
+    gamma = (1 + 0.1 * randn(320, seed=2)).to(torch.bfloat16).to(device)
+    beta = (0.1 * randn(320, seed=3)).to(torch.bfloat16).to(device)
+    w = rows(192, 320, 4, device)
+    y = ops.ln_linear_int8(x, gamma, beta, 1e-5, w, act="geglu")
+    assert torch.equal(y, ops.linear_int8(ops.ln_quantize_rows(x, gamma, beta, 1e-5), w, act="geglu"))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    bf = torch.bfloat16
+    x, w = torch.ones(4, 32, dtype=bf, device=device), rows(8, 32, 1, device)
+    i8, one = torch.zeros(4, 32, dtype=torch.int8, device=device), torch.ones(4, device=device)
+    for bad in (lambda: ops.Int8Rows(i8.float(), one), lambda: ops.Int8Rows(i8, one.double()),
+                lambda: ops.linear_int8(x, x), lambda: ops.linear_int8([1.0], w),
+                lambda: ops.quantize_rows(i8)):
+        with pytest.raises(TypeError):
+            bad()
+    odd = torch.zeros(4, 40, dtype=torch.int8, device=device)
+    for bad in (lambda: ops.Int8Rows(i8, one[:3]), lambda: ops.Int8Rows(i8[0], one),
+                lambda: ops.Int8Rows(odd[:, :32], one), lambda: ops.Int8Rows(i8[:, 1:17], one),
+                lambda: ops.Int8Rows(i8.t(), torch.ones(32, device=device)),
+                lambda: ops.Int8Rows(i8, one, (4, 31)), lambda: ops.Int8Rows(i8[:, :0], one),
+                lambda: ops.Int8Rows(torch.zeros(3 * 32 + 17, dtype=torch.int8, device=device).as_strided(
+                    (4, 17), (32, 1)), one),
+                lambda: ops.linear_int8(x[:, :16], w), lambda: ops.linear_int8(x, w, act="relu"),
+                lambda: ops.linear_int8(x, w, torch.ones(7, dtype=bf, device=device)),
+                lambda: ops.linear_int8(x, w, torch.ones(8, device=device)),
+                lambda: ops.linear_int8(x, w, residual=torch.ones(4, 7, dtype=bf, device=device)),
+                lambda: ops.linear_int8(x, w, residual=torch.ones(4, 8, dtype=bf, device=device), act="geglu"),
+                lambda: ops.linear_int8(x, rows(7, 32, 1, device), act="geglu"),
+                lambda: ops.quantize_rows(x[:, :0]), lambda: ops.quantize_rows(torch.ones((), device=device)),
+                lambda: ops.quantize_rows(torch.ones(1, ops.INT8_MAX_K + 1, dtype=bf, device=device)),
+                lambda: ops.ln_quantize_rows(x, x[0, :16], x[0], 1e-5),
+                lambda: ops.ln_quantize_rows(x, x[0].float(), x[0], 1e-5)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError, match="inference only"):
+        ops.quantize_rows(torch.ones(2, 32, dtype=bf, device=device, requires_grad=True))
+    with pytest.raises(RuntimeError, match="inference only"):
+        ops.linear_int8(x, w, torch.ones(8, dtype=bf, device=device, requires_grad=True))
+
+
+@pytest.mark.gpu
+def test_gpu_types_refused(cuda):
+    with pytest.raises(TypeError):
+        ops.quantize_rows(torch.ones(2, 32, device=cuda))
+    w = rows(8, 32, 1, cuda)
+    with pytest.raises(TypeError):
+        ops.linear_int8(ops.Int8Rows(w.q, w.scale, dtype=torch.float32), w)
+    with pytest.raises(ValueError):
+        ops.linear_int8(torch.ones(2, 32, dtype=torch.bfloat16), w)
+
+
+# ------------------------------------------------------------------ as a model uses it
+class _Block(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.ln, self.fc1, self.fc2 = layers.LayerNorm(96), layers.Linear(96, 200), layers.Linear(200, 96)
+
+    def forward(self, x):
+        return self.fc2(self.ln.linear(x, self.fc1, act="gelu"), residual=x)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layers_in_8_bits(device):
+    m = layers.init_weights(_Block(), 3).to(device=device, dtype=torch.bfloat16)
+    x = randn(2, 11, 96, seed=6, dtype=torch.bfloat16, device=device)
+    before = m(x)
+    assert layers.int8_linears(m) == 2
+    y = m(x)
+    h = ops.ln_linear_int8(x, m.ln.weight, m.ln.bias, m.ln.eps, ops.quantize_rows(m.fc1.weight), m.fc1.bias,
+                           act="gelu")
+    assert torch.equal(y, ops.linear_int8(h, ops.quantize_rows(m.fc2.weight), m.fc2.bias, residual=x))
+    # 8-bit weights and activations: each operand is off by at most half of 1/127 of its row's largest value
+    assert (y.float() - before.float()).norm() < 0.03 * before.float().norm()
+    layers.int8_linears(m, False)
+    assert torch.equal(m(x), before)
+
+
+@pytest.mark.gpu
+def test_streams_and_graph_replays(cuda):
+    x = randn(33, 640, seed=1, dtype=torch.bfloat16, device=cuda)
+    w, b = rows(384, 640, 2, cuda), randn(384, seed=3, dtype=torch.bfloat16, device=cuda)
+    want = ops.linear_int8(x, w, b, act="geglu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.linear_int8(x, w, b, act="geglu")
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    xs, graphs = [x.clone(), x.clone()], []
+    for i in range(2):                    # two graphs of the same weight, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.linear_int8(xs[i], w, b, act="geglu")
+        graphs.append((g, y))
+    for step in range(4):
+        for i in range(2):
+            xs[i].copy_(randn(33, 640, seed=10 * step + i, dtype=torch.bfloat16, device=cuda))
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(graphs[i][1], ops.linear_int8(xs[i], w, b, act="geglu"))
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_grid_dimension(cuda):
+    m = 70001
+    x = randn(64, 48, seed=1, dtype=torch.bfloat16, device=cuda).repeat(-(-m // 64), 1)[:m]
+    w = rows(40, 48, 2, cuda)
+    y = ops.linear_int8(x, w)
+    assert torch.equal(y[:64].repeat(-(-m // 64), 1)[:m], y)

@@ -1,0 +1,390 @@
+"""``ops.masked_attention`` against its definition in 64 bits (masks built key by key), on the CPU reference and on
+the HIP kernels.
+
+Tolerance.  With w the exact softmax weights, V = sum_j w_j |v_j|: the weights enter the second product
+rounded to the input type (half a step each, u = finfo.eps / 2), scores are fp32 sums of exact products and are
+off by less than 2^-13 here (|scale q.k| < 64, cap tanh within cap 2^-21), which moves a weight by 2^-12 of
+itself at most; the output is rounded once: |o - ref| <= (u + 2^-12) V + u |ref| (+ 2^-25 in fp16's subnormals)."""
+import math
+
+import pytest
+import torch
+
+from arbius_amd import ops
+from arbius_amd.models import layers
+from arbius_amd.models.clip_text import CLIPTextConfig, CLIPTextEncoder
+from arbius_amd.models.xlmr import MCLIPText, XLMRConfig
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def randn(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def seen_keys(b, i, nk, o):
+    """The keys query i of batch row b sees, from the masks' definitions."""
+    start = o.get("q_start", 0)
+    p = (int(start[b]) if isinstance(start, torch.Tensor) else start) + i
+    docs, prefix, lengths = o.get("documents"), o.get("prefix"), o.get("lengths")
+    ok = torch.ones(nk, dtype=torch.bool)
+    j = torch.arange(nk)
+    first, shown = 0, None
+    if docs is not None:
+        off = (docs[b] if docs.dim() == 2 else docs).tolist()
+        t = [t for t in range(len(off) - 1) if off[t] <= p < off[t + 1]]
+        if not t:
+            return ~ok, p
+        first = off[t[0]]
+        ok &= (j >= first) & (j < off[t[0] + 1])
+        if prefix is not None:
+            shown = int((prefix[b] if prefix.dim() == 2 else prefix)[t[0]])
+    elif prefix is not None:
+        shown = int(prefix[b])
+    if o.get("causal"):
+        ok &= (j <= p) | ((j < first + shown) if shown is not None else torch.zeros_like(ok))
+    if lengths is not None:
+        ok &= j < int(lengths[b])
+    return ok, p
+
+
+def definition(q, k, v, o):
+    B, Nq, H, D = q.shape
+    Nk, group = k.shape[1], H // k.shape[2]
+    scale = o.get("scale") or 1.0 / math.sqrt(D)
+    out, mag = torch.zeros(B, Nq, H, D, dtype=torch.float64), torch.zeros(B, Nq, H, D, dtype=torch.float64)
+    j = torch.arange(Nk)
+    for b in range(B):
+        runs = [seen_keys(b, i, Nk, o) for i in range(Nq)]
+        ok = torch.stack([r[0] for r in runs])
+        p = torch.tensor([r[1] for r in runs])
+        some = ok.any(dim=1)
+        for h in range(H):
+            kk = k[b, :, h // group].double()
+            vv = v[b, :, h // group].double()
+            s = (q[b, :, h].double() @ kk.t()) * scale
+            if o.get("softcap"):
+                s = o["softcap"] * torch.tanh(s / o["softcap"])
+            if o.get("slopes") is not None:
+                s = s - o["slopes"][h].double() * (p[:, None] - j).abs()
+            s = torch.where(ok, s, torch.full_like(s, -math.inf))[some]
+            w = torch.softmax(s, dim=1)
+            used = ok.any(dim=0)                      # values no query sees stay out
+            out[b, some, h] = w[:, used] @ vv[used]
+            mag[b, some, h] = w[:, used] @ vv[used].abs()
+    return out, mag
+
+
+def check(y, want, mag):
+    u = torch.finfo(y.dtype).eps / 2
+    y = y.cpu().double()
+    assert not bool(y.isnan().any())
+    over = (y - want).abs() - ((u + 2.0 ** -12) * mag + u * want.abs() + 2.0 ** -25)
+    assert bool((over <= 0).all()), f"over the bound by {over.max().item():.3g}"
+
+
+def to(device, o):
+    return {n: t.to(device) if isinstance(t, torch.Tensor) else t for n, t in o.items()}
+
+
+def run(q, k, v, o, device):
+    return ops.masked_attention(q.to(device), k.to(device), v.to(device), **to(device, o))
+
+
+def slopes(H):
+    return 2.0 ** (-8.0 * torch.arange(1, H + 1, dtype=torch.float32) / H)
+
+
+CASES = {
+    "plain": dict(shape=(2, 77, 77, 3, 3, 64)),
+    "one": dict(shape=(1, 1, 1, 1, 1, 8)),
+    "one key": dict(shape=(2, 70, 1, 2, 2, 32)),
+    "one query": dict(shape=(3, 1, 200, 4, 2, 64), q_start=199, causal=True),
+    "wide head": dict(shape=(1, 40, 70, 2, 1, 256), causal=True),
+    "head 40": dict(shape=(2, 33, 65, 4, 4, 40)),
+    "head 80": dict(shape=(1, 129, 129, 2, 2, 80), causal=True),
+    "head 96": dict(shape=(1, 64, 64, 2, 2, 96), softcap=5.0),
+    "head 160": dict(shape=(1, 100, 100, 2, 1, 160), causal=True, slopes=slopes(2)),
+    "head 200": dict(shape=(1, 50, 131, 2, 2, 200)),
+    "groups": dict(shape=(2, 61, 61, 8, 2, 64), causal=True),
+    "groups of 3": dict(shape=(1, 90, 90, 6, 2, 32), causal=True, slopes=slopes(6), softcap=20.0),
+    "multi-query": dict(shape=(2, 5, 300, 16, 1, 128), causal=True, q_start=295),
+    "lengths": dict(shape=(6, 77, 77, 2, 2, 64), lengths=i32([0, 1, 5, 63, 64, 77])),
+    "lengths past the end": dict(shape=(3, 20, 20, 2, 2, 64), lengths=i32([-5, 1000, 2 ** 31 - 1])),
+    "causal lengths": dict(shape=(3, 150, 150, 2, 2, 64), causal=True, lengths=i32([10, 0, 150])),
+    "prefix": dict(shape=(4, 140, 140, 2, 2, 64), causal=True, prefix=i32([0, 1, 70, 140])),
+    "prefix past the end": dict(shape=(2, 30, 30, 2, 2, 64), causal=True, prefix=i32([-3, 2 ** 31 - 1])),
+    "documents": dict(shape=(1, 300, 300, 2, 2, 64), documents=i32([0, 5, 64, 64, 65, 200, 300])),
+    "documents causal": dict(shape=(1, 300, 300, 2, 2, 64), causal=True, documents=i32([0, 5, 64, 65, 200, 300])),
+    "documents with gaps": dict(shape=(1, 200, 200, 2, 2, 64), documents=i32([7, 30, 130])),
+    "documents past the end": dict(shape=(1, 100, 100, 2, 2, 64), documents=i32([0, 60, 400])),
+    "documents per row": dict(shape=(2, 90, 90, 2, 2, 64), documents=i32([[0, 40, 90], [10, 20, 70]])),
+    "documents prefix": dict(shape=(1, 160, 160, 2, 2, 64), causal=True, documents=i32([0, 50, 120, 160]),
+                             prefix=i32([10, 0, 1000])),
+    "documents prefix per row": dict(shape=(2, 80, 80, 2, 2, 64), causal=True, documents=i32([0, 50, 80]),
+                                     prefix=i32([[10, 0], [3, 9]])),
+    "documents lengths": dict(shape=(2, 90, 90, 2, 2, 64), documents=i32([0, 40, 90]), lengths=i32([60, 20])),
+    "one document": dict(shape=(1, 70, 70, 1, 1, 64), documents=i32([0, 70])),
+    "softcap": dict(shape=(2, 100, 100, 2, 2, 64), causal=True, softcap=2.0),
+    "softcap 50 far over it": dict(shape=(1, 80, 80, 2, 2, 64), softcap=50.0, scale=3.0),
+    "slopes": dict(shape=(2, 130, 130, 4, 4, 64), slopes=slopes(4)),
+    "rising slopes": dict(shape=(1, 66, 66, 2, 2, 64), causal=True, slopes=torch.tensor([-0.05, 0.0])),
+    "starts": dict(shape=(4, 3, 257, 4, 2, 64), causal=True, q_start=i32([0, 100, 254, 300]), slopes=slopes(4)),
+    "starts before the first key": dict(shape=(2, 4, 40, 2, 2, 64), causal=True, q_start=i32([-2, -100])),
+    "start past every key": dict(shape=(1, 4, 40, 2, 2, 64), causal=True, q_start=2 ** 31 - 5),
+    "cached rows": dict(shape=(4, 2, 700, 8, 2, 128), causal=True, q_start=i32([10, 400, 0, 698]),
+                        lengths=i32([12, 402, 2, 700])),
+    "long cache, few rows": dict(shape=(1, 1, 5003, 4, 2, 64), causal=True, q_start=5002, slopes=slopes(4)),
+    "long cache, short lengths": dict(shape=(2, 1, 5000, 4, 2, 64), lengths=i32([0, 130]), softcap=30.0),
+    "all": dict(shape=(2, 190, 190, 6, 3, 80), causal=True, documents=i32([3, 90, 180]), prefix=i32([20, 5]),
+                lengths=i32([190, 100]), softcap=10.0, slopes=slopes(6), scale=0.2),
+}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", CASES)
+def test_against_the_definition(device, dtype, name):
+    o = dict(CASES[name])
+    B, Nq, Nk, H, Hkv, D = o.pop("shape")
+    dt = DTYPES[dtype]
+    q, k, v = randn(B, Nq, H, D, seed=1, dtype=dt), randn(B, Nk, Hkv, D, seed=2, dtype=dt), \
+        randn(B, Nk, Hkv, D, seed=3, dtype=dt)
+    y = run(q, k, v, o, device)
+    assert y.dtype == dt and tuple(y.shape) == (B, Nq, H, D)
+    check(y, *definition(q, k, v, o))
+
+
+POISONED = {
+    "lengths": dict(shape=(3, 70, 200, 2, 2, 64), lengths=i32([0, 64, 131])),
+    "documents": dict(shape=(1, 210, 210, 2, 1, 64), documents=i32([0, 50, 130, 150])),
+    "cache": dict(shape=(3, 1, 4000, 4, 2, 128), causal=True, q_start=i32([0, 77, 3000]), lengths=i32([1, 78, 2001])),
+    "causal": dict(shape=(1, 100, 300, 2, 2, 80), causal=True),
+}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", ["nan", "inf", "lowest"])
+@pytest.mark.parametrize("name", POISONED)
+def test_masked_places_may_hold_anything(device, dtype, bad, name):
+    o = dict(POISONED[name])
+    B, Nq, Nk, H, Hkv, D = o.pop("shape")
+    dt = DTYPES[dtype]
+    val = {"nan": float("nan"), "inf": float("inf"), "lowest": torch.finfo(dt).min}[bad]
+    q, k, v = randn(B, Nq, H, D, seed=1, dtype=dt), randn(B, Nk, Hkv, D, seed=2, dtype=dt), \
+        randn(B, Nk, Hkv, D, seed=3, dtype=dt)
+    clean = run(q, k, v, o, device)
+    for b in range(B):
+        unseen = ~torch.stack([seen_keys(b, i, Nk, o)[0] for i in range(Nq)]).any(dim=0)
+        k[b, unseen], v[b, unseen] = val, val
+    y = run(q, k, v, o, device)
+    assert not bool(y.isnan().any()) and torch.equal(y, clean)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("val", [float("nan"), float("inf"), -float("inf")])
+def test_a_value_reaches_only_the_queries_that_see_it(device, val):
+    """V row 50 of a causal row set, V row 20 of one document: queries before it / of the others stay clean."""
+    q, k, v = (randn(1, 140, 2, 64, seed=s, dtype=torch.bfloat16) for s in (1, 2, 3))
+    at_i = torch.arange(140)
+    for o, at, hit in ((dict(causal=True), 50, at_i >= 50),
+                       (dict(documents=i32([0, 10, 30, 140])), 20, (at_i >= 10) & (at_i < 30))):
+        clean = run(q, k, v, o, device).cpu()
+        w = v.clone()
+        w[0, at, 0, 5] = val
+        y = run(q, k, w, o, device).cpu()
+        rest = torch.ones_like(clean, dtype=torch.bool)
+        rest[0, hit, 0, 5] = False
+        assert torch.equal(y[rest], clean[rest])
+        got = y[0, hit, 0, 5]
+        assert bool(got.isnan().all()) if math.isnan(val) else bool((got == val).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_nan_key_or_query_stays_with_its_rows(device):
+    q, k, v = (randn(1, 80, 2, 64, seed=s, dtype=torch.bfloat16) for s in (1, 2, 3))
+    clean = run(q, k, v, dict(causal=True), device).cpu()
+    k2, q2 = k.clone(), q.clone()
+    k2[0, 70, 1], q2[0, 33, 0, 3] = float("nan"), float("nan")
+    y = run(q2, k2, v, dict(causal=True), device).cpu()
+    assert bool(y[0, 70:, 1].isnan().all()) and bool(y[0, 33, 0].isnan().all())
+    y[0, 70:, 1], y[0, 33, 0] = clean[0, 70:, 1], clean[0, 33, 0]
+    assert torch.equal(y, clean)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_strided_views(device):
+    qkv = randn(2, 90, 3, 4, 64, seed=5, dtype=torch.bfloat16).to(device)
+    o = dict(causal=True, lengths=i32([90, 31]))
+    y = ops.masked_attention(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], **to(device, o))
+    assert torch.equal(y, ops.masked_attention(*(qkv[:, :, i].contiguous() for i in range(3)), **to(device, o)))
+    # head-major caches, and one key / value set shared by every batch row
+    kh, vh = (randn(2, 2, 90, 64, seed=s, dtype=torch.bfloat16).to(device).transpose(1, 2) for s in (6, 7))
+    y = ops.masked_attention(qkv[:, :, 0], kh, vh, **to(device, o))
+    assert torch.equal(y, ops.masked_attention(qkv[:, :, 0].contiguous(), kh.contiguous(), vh.contiguous(),
+                                               **to(device, o)))
+    ke, ve = kh[:1].expand(2, -1, -1, -1), vh[:1].expand(2, -1, -1, -1)
+    y = ops.masked_attention(qkv[:, :, 0], ke, ve, causal=True)
+    assert torch.equal(y, ops.masked_attention(qkv[:, :, 0], ke.contiguous(), ve.contiguous(), causal=True))
+    # index tensors that are columns or rows of others
+    both = i32([[90, 1], [31, 2]]).to(device)
+    with pytest.raises(ValueError):
+        ops.masked_attention(qkv[:, :, 0], kh, vh, lengths=both[:, 0])
+    docs = i32([[0, 40, 90, 7], [5, 6, 60, 7]]).to(device)[:, :3]
+    y = ops.masked_attention(qkv[:, :, 0], kh, vh, documents=docs)
+    assert torch.equal(y, ops.masked_attention(qkv[:, :, 0], kh, vh, documents=docs.contiguous()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_batch_rows_do_not_touch_each_other(device):
+    q, k, v = (randn(8, 100, 4, 64, seed=s, dtype=torch.bfloat16).to(device) for s in (1, 2, 3))
+    n = i32([100, 3, 77, 64, 65, 1, 50, 99]).to(device)
+    y = ops.masked_attention(q, k, v, lengths=n, causal=True, slopes=slopes(4).to(device))
+    with ops.plan_batch(1):
+        group = ops.masked_attention(q, k, v, lengths=n, causal=True, slopes=slopes(4).to(device))
+        for b in range(8):
+            one = ops.masked_attention(q[b:b + 1], k[b:b + 1], v[b:b + 1], lengths=n[b:b + 1], causal=True,
+                                       slopes=slopes(4).to(device))
+            assert torch.equal(one[0], group[b])
+    assert torch.equal(y, ops.masked_attention(q, k, v, lengths=n, causal=True, slopes=slopes(4).to(device)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_empty_shapes(device):
+    q, k = torch.ones(2, 3, 4, 64, dtype=torch.bfloat16, device=device), \
+        torch.ones(2, 0, 2, 64, dtype=torch.bfloat16, device=device)
+    assert not bool(ops.masked_attention(q, k, k).any())
+    assert tuple(ops.masked_attention(q[:, :0], k, k).shape) == (2, 0, 4, 64)
+    assert tuple(ops.masked_attention(q[:0], k[:0], k[:0]).shape) == (0, 3, 4, 64)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    q, k = torch.ones(2, 3, 4, 64, dtype=torch.bfloat16, device=device), \
+        torch.ones(2, 5, 2, 64, dtype=torch.bfloat16, device=device)
+    n, att = i32([1, 2]).to(device), ops.masked_attention
+    for bad in (lambda: att(q[0], k, k), lambda: att(q, k, k[:, :4]), lambda: att(q[:1], k, k),
+                lambda: att(q[..., :32], k, k), lambda: att(q[:, :, :3], k, k),
+                lambda: att(q, k, k, scale=float("nan")), lambda: att(q, k, k, softcap=0.0),
+                lambda: att(q, k, k, softcap=-1.0), lambda: att(q, k, k, softcap=float("inf")),
+                lambda: att(q, k, k, q_start=-1), lambda: att(q, k, k, q_start=2 ** 31),
+                lambda: att(q, k, k, lengths=n[:1]), lambda: att(q, k, k, q_start=n[:1]),
+                lambda: att(q, k, k, documents=n[:1]), lambda: att(q, k, k, documents=n[:0]),
+                lambda: att(q, k, k, documents=n[0]), lambda: att(q, k, k, prefix=n),
+                lambda: att(q, k, k, causal=True, prefix=n[:1]),
+                lambda: att(q, k, k, causal=True, documents=n, prefix=n),
+                lambda: att(q, k, k, slopes=slopes(2).to(device)), lambda: att(q, k, k, slopes=0.5),
+                lambda: att(q, k, k, slopes=slopes(4).double().to(device))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: att(q, k.half(), k), lambda: att(q, k, k, lengths=n.long()),
+                lambda: att(q, k, k, lengths=[1, 2]), lambda: att(q, k, k, causal=True, prefix=n.float())):
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(RuntimeError, match="inference only"):
+        att(q.clone().requires_grad_(), k, k)
+
+
+@pytest.mark.gpu
+def test_gpu_refusals(cuda):
+    q = torch.ones(1, 3, 2, 72, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(TypeError):
+        ops.masked_attention(q.float(), q.float(), q.float())
+    for t in (q[..., :4], q[..., 4:], torch.ones(1, 3, 2, 264, dtype=torch.bfloat16, device=cuda)):
+        with pytest.raises(ValueError):
+            ops.masked_attention(t, t, t)
+    with pytest.raises(ValueError):
+        ops.masked_attention(q[..., :64].transpose(1, 3), q, q)
+    with pytest.raises(TypeError):
+        ops.masked_attention(q, q, q, lengths=i32([3]))
+
+
+@pytest.mark.gpu
+def test_cache_past_32_bit_offsets(cuda):
+    """A cache whose last keys lie more than 2^32 bytes behind its first."""
+    n, row = 70000, 32768
+    store = torch.empty(n, row, dtype=torch.bfloat16, device=cuda)
+    k, v = store[None, :, :128].view(1, n, 2, 64), store[None, :, 4096:4224].view(1, n, 2, 64)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    for t in (store[:, :128], store[:, 4096:4224]):
+        t.copy_(torch.randn(n, 128, generator=gen, device=cuda))
+    q = torch.randn(1, 2, 4, 64, generator=gen, device=cuda).to(torch.bfloat16)
+    o = dict(causal=True, q_start=n - 2, slopes=torch.tensor([0.0, 2.0 ** -12, 0.5, 0.0]))
+    y = run(q, k, v, o, cuda)
+    assert torch.equal(y, run(q, k.contiguous(), v.contiguous(), o, cuda))
+    check(y, *definition(q.cpu(), k.cpu(), v.cpu(), o))
+
+
+@pytest.mark.gpu
+def test_many_batch_rows(cuda):
+    B = 70000
+    q, k, v = (randn(64, n, 1, 32, seed=s, dtype=torch.bfloat16).to(cuda).repeat(-(-B // 64), 1, 1, 1)[:B]
+               for s, n in ((1, 2), (2, 5), (3, 5)))
+    y = ops.masked_attention(q, k, v, lengths=torch.full((B,), 4, dtype=torch.int32, device=cuda))
+    check(y[:64], *definition(q[:64].cpu(), k[:64].cpu(), v[:64].cpu(), dict(lengths=i32([4] * 64))))
+    assert torch.equal(y, y[:64].repeat(-(-B // 64), 1, 1, 1)[:B])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nk", [(100, 100), (1, 6000)])
+def test_streams_and_graph_replays(cuda, nq, nk):
+    """Two graphs over caches that grow between replays; lengths and positions are read on the device."""
+    q = [randn(2, nq, 4, 64, seed=s, dtype=torch.bfloat16).to(cuda) for s in (1, 2)]
+    k, v = (randn(2, nk, 2, 64, seed=s, dtype=torch.bfloat16).to(cuda) for s in (3, 4))
+    n, start = i32([nk, 1]).to(cuda), i32([0, 0]).to(cuda)
+    o = dict(causal=True, lengths=n, q_start=start, softcap=20.0)
+    want = ops.masked_attention(q[0], k, v, **o)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.masked_attention(q[0], k, v, **o)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.masked_attention(q[i], k, v, **o)
+        graphs.append((g, y))
+    for step in range(1, 5):
+        n.copy_(i32([nk // step, step * nk // 5]))
+        start.copy_(i32([max(0, nk // step - nq), step]))
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(graphs[i][1], ops.masked_attention(q[i], k, v, **o))
+
+
+# ------------------------------------------------------------------ as the text towers use it
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("int8", [False, True])
+def test_packed_prompts_through_the_text_towers(device, int8):
+    """Prompts packed end to end give what each gives alone: a run of 8-bit linears and masked attention."""
+    dt = torch.bfloat16 if device == "cuda" else torch.float32
+    lens = [5, 30, 1, 77, 12]
+    off = i32([0] + list(torch.tensor(lens).cumsum(0)))
+    ids = torch.randint(3, 900, (sum(lens),), generator=torch.Generator().manual_seed(1))
+    clip = layers.init_weights(CLIPTextEncoder(CLIPTextConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256)), 1)
+    xlmr = layers.init_weights(MCLIPText(XLMRConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256, max_pos=100,
+                                                    proj_dim=64)), 2)
+    for model in (clip, xlmr):
+        model.to(device=device, dtype=dt).eval()
+        ids[off[1:].long() - 1] = 999                       # every prompt ends with its EOS
+        if int8:
+            assert layers.int8_linears(model) == (8 if model is clip else 9)
+        full, pooled = model.forward_packed(ids.to(device), off.to(device))
+        for t, n in enumerate(lens):
+            row = ids[int(off[t]):int(off[t + 1])][None].to(device)
+            one, pool = model(row) if model is clip else model(row, n)
+            part = full[int(off[t]):int(off[t + 1])]
+            # bf16: two layers of roundings at 2^-8 each, an 8-bit step where one flips; fp32: sums in another order
+            tol = 2e-4 if dt == torch.float32 and not int8 else 0.03
+            assert (part.float() - one[0].float()).norm() <= tol * one[0].float().norm()
+            assert (pooled[t].float() - pool[0].float()).norm() <= tol * pool[0].float().norm()
