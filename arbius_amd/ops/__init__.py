@@ -821,8 +821,8 @@ def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=No
         raise ValueError(f"masked_attention: slopes must be contiguous fp32 [{H}] on {q.device}")
     if Nq >= 2 ** 31 or k.shape[1] >= 2 ** 31:
         raise ValueError("masked_attention: more than 2^31 - 1 queries or keys")
-    impl = _lib if _hip(q) else ref
-    return impl.masked_attention(q, k, v, scale, bool(causal), q_start, lengths, prefix, documents, softcap, slopes)
+    args = (q, k, v, scale, bool(causal), q_start, lengths, prefix, documents, softcap, slopes)
+    return _lib.masked_attention(*args, _canon_batch(B)) if _hip(q) else ref.masked_attention(*args)
 
 
 # --------------------------------------------------------------------------- ConvGRU

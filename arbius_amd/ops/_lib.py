@@ -94,7 +94,8 @@ _SIGS = {
                                   c_int, c_int, c_void_p]),
     "arb_linear_int8": (c_int, [c_void_p, c_long, c_void_p, c_void_p, c_long] + [c_void_p] * 4 + [c_int] * 5
                         + [c_void_p]),
-    "arb_masked_attention": (c_int, [c_void_p] * 11 + [c_float, c_float, c_int, c_void_p]),
+    "arb_masked_attention": (c_int, [c_void_p] * 12 + [c_float, c_float, c_int, c_void_p]),
+    "arb_masked_attention_workspace": (c_size_t, [c_int, c_long] + [c_int] * 5),
 }
 
 
@@ -134,7 +135,7 @@ _AUDIT = None
 _HOST_SYMBOLS = ("arb_conv2d_plan", "arb_conv_family", "arb_conv2d_workspace", "arb_group_norm_workspace",
                  "arb_group_norm_slice_ok",
                  "arb_rvm_args_sizes", "arb_attention512_workspace", "arb_h264_intra_workspace",
-                 "arb_h264_intra_host")
+                 "arb_h264_intra_host", "arb_masked_attention_workspace")
 
 
 def auditing() -> bool:
@@ -1176,8 +1177,9 @@ def linear_int8(q, sx, w, sw, b, residual, act, shape, dtype):
     return y
 
 
-def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents, softcap, slopes):
-    """Arguments as checked by ``ops.masked_attention`` (csrc/masked_attention.hip)."""
+def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents, softcap, slopes, plan_b=None):
+    """Arguments as checked by ``ops.masked_attention`` (csrc/masked_attention.hip).  plan_b: the canonical batch
+    the key split is chosen for (default: the actual one)."""
     el = _el("masked_attention", q)
     B, Nq, H, D = q.shape
     Nk, Hkv = k.shape[1], k.shape[2]
@@ -1186,6 +1188,8 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
     for t in (q, k, v):
         if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
             raise ValueError("masked_attention: last dim must be contiguous, strides/base 16B aligned")
+    # keys that share memory (a token stride below D) or lie 16 MiB apart are out of the tile loads' addressing
+    k, v = (t if D <= t.stride(1) < 1 << 23 else t.contiguous() for t in (k, v))
     o = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
     if not o.numel():
         return o
@@ -1195,10 +1199,13 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
     docs_sb = documents.stride(0) if documents is not None and documents.dim() == 2 else 0
     prefix_sb = 0 if prefix is None else prefix.stride(0) if documents is None or prefix.dim() == 2 else 0
     strides = (c_long * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
-    ints = (c_long * 11)(B, H, Hkv, Nq, Nk, D, int(causal), 0 if starts else q_start,
-                         0 if documents is None else documents.shape[-1] - 1, docs_sb, prefix_sb)
+    plan_b = plan_b or B
+    ints = (c_long * 12)(B, H, Hkv, Nq, Nk, D, int(causal), 0 if starts else q_start,
+                         0 if documents is None else documents.shape[-1] - 1, docs_sb, prefix_sb, plan_b)
+    wsb = _fn("arb_masked_attention_workspace")(B, plan_b, H, Hkv, Nq, Nk, D)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
     with _on(q) as stream:
         _check(_fn("arb_masked_attention")(_p(q), _p(k), _p(v), _p(o), strides, ints, _p(q_start if starts else None),
-                                           _p(lengths), _p(documents), _p(prefix), _p(slopes), float(scale),
+                                           _p(lengths), _p(documents), _p(prefix), _p(slopes), _p(ws), float(scale),
                                            float(softcap or 0.0), el, stream), "masked_attention")
     return o
