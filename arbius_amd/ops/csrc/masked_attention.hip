@@ -502,7 +502,8 @@ __global__ void __launch_bounds__(256) masked_attention_join_kernel(MaskedArgs a
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int r = (int)(at % R), hk = (int)(at / R % a.Hkv), b = (int)(at / R / a.Hkv), i = r / G;
   uint16_t* o = a.o + b * a.o_sb + i * a.o_sn + (hk * G + r - i * G) * a.o_sh + d;
-  *reinterpret_cast<uint2*>(o) = make_uint2(pack2<EL>(acc[0] * inv, acc[1] * inv), pack2<EL>(acc[2] * inv, acc[3] * inv));
+  *reinterpret_cast<uint2*>(o) =
+      make_uint2(pack2<EL>(acc[0] * inv, acc[1] * inv), pack2<EL>(acc[2] * inv, acc[3] * inv));
 }
 
 template <int EL, int DC, int QT>
