@@ -319,18 +319,19 @@ class Int8Rows:
     def __init__(self, q, scale, shape=None, dtype=torch.bfloat16):
         if q.dtype != torch.int8 or scale.dtype != torch.float32 or q.device != scale.device:
             raise TypeError("Int8Rows: q int8 and scale fp32 on one device")
-        if q.dim() != 2 or tuple(scale.shape) != (q.shape[0],) or not scale.is_contiguous():
+        if q.dim() != 2 or scale.shape != q.shape[:1] or not scale.is_contiguous():
             raise ValueError(f"Int8Rows: q {tuple(q.shape)} scale {tuple(scale.shape)} (q [R, K], scale [R])")
         R, K = q.shape
-        shape = (R, K) if shape is None else tuple(shape)
-        if not 1 <= K <= INT8_MAX_K or shape[-1] != K or math.prod(shape[:-1]) != R:
+        if not 1 <= K <= INT8_MAX_K or (shape is not None and (shape[-1] != K or math.prod(shape[:-1]) != R)):
             raise ValueError(f"Int8Rows: q {tuple(q.shape)} for shape {shape} (1 <= K <= {INT8_MAX_K})")
         pad = -(-K // 16) * 16
-        if q.stride(1) != 1 or (R and (q.data_ptr() % 16 or q.stride(0) % 16 or q.stride(0) < pad)):
+        ld, one = q.stride()
+        if R and (one != 1 or q.data_ptr() % 16 or ld % 16 or ld < pad):
             raise ValueError(f"Int8Rows: rows need stride >= {pad} and, like the base, a multiple of 16 bytes")
-        if R and q.storage_offset() + (R - 1) * q.stride(0) + pad > q.untyped_storage().nbytes():
+        if R and pad != K and q.storage_offset() + (R - 1) * ld + pad > q.untyped_storage().nbytes():
             raise ValueError("Int8Rows: the storage ends inside the last row's padding")
-        self.q, self.scale, self.shape, self.dtype = q, scale, shape, dtype
+        self.q, self.scale, self.dtype = q, scale, dtype
+        self.shape = (R, K) if shape is None else tuple(shape)
         self.zero_tail = pad == K
 
     @property
@@ -371,10 +372,17 @@ def quantize_rows(x):
 
 def ln_quantize_rows(x, gamma, beta, eps):
     """``quantize_rows`` of LayerNorm(x), the normalised row held in fp32 until it is quantised."""
+    return _quantize(x, _norm_args(x, gamma, beta, eps, "ln_quantize_rows"), "ln_quantize_rows")
+
+
+def _norm_args(x, gamma, beta, eps, op):
+    want, dtype, device = x.shape[-1:], x.dtype, x.device
     for t in (gamma, beta):
-        if tuple(t.shape) != (x.shape[-1],) or t.dtype != x.dtype or t.device != x.device or not t.is_contiguous():
-            raise ValueError(f"ln_quantize_rows: gamma / beta must be contiguous {x.dtype} [{x.shape[-1]}]")
-    return _quantize(x, (gamma, beta, float(eps)), "ln_quantize_rows")
+        if t.shape != want or t.dtype != dtype or t.device != device or not t.is_contiguous():
+            raise ValueError(f"{op}: gamma / beta must be contiguous {x.dtype} {list(want)}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{op}: inference only (no gradients)")
+    return gamma, beta, float(eps)
 
 
 def linear_int8(x, w, b=None, residual=None, act=None):
@@ -385,40 +393,64 @@ def linear_int8(x, w, b=None, residual=None, act=None):
 
     The integer sums are exact, so y does not depend on tiles, splits or the other rows of the batch.
     GPU: b, residual and y in x's dtype (bf16 / fp16) (csrc/linear_int8.hip).  Inference only."""
-    if not isinstance(w, Int8Rows) or len(w.shape) != 2:
-        raise TypeError("linear_int8: w must be the Int8Rows of a weight [N, K]")
-    if not isinstance(x, (torch.Tensor, Int8Rows)):
-        raise TypeError(f"linear_int8: x is a {type(x).__name__}")
-    N, K = w.shape
-    if x.shape[-1] != K or x.device != w.device:
-        raise ValueError(f"linear_int8: x {tuple(x.shape)} on {x.device}, w {w.shape} on {w.device}")
-    if act not in _lib._INT8_ACT:
-        raise ValueError(f"linear_int8: act {act!r}")
-    if act == "geglu" and (N % 2 or residual is not None):
-        raise ValueError("linear_int8: geglu needs an even number of weight rows and takes no residual")
-    shape = tuple(x.shape[:-1])
-    for name, t, want in (("b", b, (N,)), ("residual", residual, shape + (N,))):
-        if t is None:
-            continue
-        if tuple(t.shape) != want or t.dtype != x.dtype or t.device != w.device:
-            raise ValueError(f"linear_int8: {name} {tuple(t.shape)} {t.dtype}, {want} {x.dtype} expected")
-        if torch.is_grad_enabled() and t.requires_grad:
-            raise RuntimeError("linear_int8: inference only (no gradients)")
-    b = None if b is None else b.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    rows = x if isinstance(x, Int8Rows) else quantize_rows(x)
-    q = rows.q
-    if not rows.zero_tail:               # the caller's own rows: what follows column K must not reach the sums
-        q = F.pad(q, (0, -K % 16))[:, :K]
+    if not isinstance(x, Int8Rows):
+        return _linear_int8(x, None, w, b, residual, act, "linear_int8")
+    shape, b, residual = _linear_int8_args(x, x.shape, w, b, residual, act, "linear_int8")
+    q = x.q
+    if not x.zero_tail:                  # the caller's own rows: what follows column K must not reach the sums
+        q = F.pad(q, (0, -x.shape[-1] % 16))[:, :x.shape[-1]]
     impl = _lib if _hip(w.q) else ref
-    if impl is _lib and rows.dtype not in _lib._EL:
-        raise TypeError(f"linear_int8: the HIP kernel writes bf16 or fp16, not {rows.dtype}")
-    return impl.linear_int8(q, rows.scale, w.q, w.scale, b, residual, act, shape, rows.dtype)
+    return impl.linear_int8(q, x.scale, w.q, w.scale, b, residual, act, shape, x.dtype)
+
+
+def _linear_int8_args(x, xshape, w, b, residual, act, op):
+    if not isinstance(w, Int8Rows) or len(w.shape) != 2:
+        raise TypeError(f"{op}: w must be the Int8Rows of a weight [N, K]")
+    N, K = w.shape
+    device, shape = w.q.device, tuple(xshape[:-1])
+    if xshape[-1] != K or x.device != device:
+        raise ValueError(f"{op}: x {tuple(xshape)} on {x.device}, w {w.shape} on {device}")
+    if act is not None and act not in _lib._INT8_ACT:
+        raise ValueError(f"{op}: act {act!r}")
+    if act == "geglu" and (N % 2 or residual is not None):
+        raise ValueError(f"{op}: geglu needs an even number of weight rows and takes no residual")
+    grad = torch.is_grad_enabled()
+    if b is not None:
+        if b.shape != (N,) or b.dtype != x.dtype or b.device != device:
+            raise ValueError(f"{op}: b {tuple(b.shape)} {b.dtype}, [{N}] {x.dtype} expected")
+        if grad and b.requires_grad:
+            raise RuntimeError(f"{op}: inference only (no gradients)")
+        b = b.contiguous()
+    if residual is not None:
+        if residual.shape != (*shape, N) or residual.dtype != x.dtype or residual.device != device:
+            raise ValueError(f"{op}: residual {tuple(residual.shape)} {residual.dtype}, {(*shape, N)} {x.dtype} "
+                             "expected")
+        if grad and residual.requires_grad:
+            raise RuntimeError(f"{op}: inference only (no gradients)")
+        residual = residual.contiguous()
+    return shape, b, residual
+
+
+def _linear_int8(x, norm, w, b, residual, act, op):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{op}: x is a {type(x).__name__}")
+    xshape = x.shape
+    if not xshape:
+        raise ValueError(f"{op}: x has no dimensions")
+    shape, b, residual = _linear_int8_args(x, xshape, w, b, residual, act, op)
+    if not x.is_floating_point():
+        raise TypeError(f"{op}: got {x.dtype}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{op}: inference only (no gradients)")
+    if _hip(x):
+        return _lib.linear_int8_of(x, norm, w.q, w.scale, b, residual, act)
+    rows = _quantize(x, norm, op)
+    return ref.linear_int8(rows.q, rows.scale, w.q, w.scale, b, residual, act, shape, rows.dtype)
 
 
 def ln_linear_int8(x, gamma, beta, eps, w, b=None, residual=None, act=None):
     """``linear_int8`` of LayerNorm(x): normalised and quantised in one pass over x."""
-    return linear_int8(ln_quantize_rows(x, gamma, beta, eps), w, b, residual, act)
+    return _linear_int8(x, _norm_args(x, gamma, beta, eps, "ln_linear_int8"), w, b, residual, act, "ln_linear_int8")
 
 
 class CatPair:
@@ -758,7 +790,7 @@ TEMPORAL_MAX_FRAMES = 96     # csrc/temporal_attention.hip keeps <= 96 frames in
 def _index_arg(name, t, like, shapes):
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != like.device:
         raise TypeError(f"masked_attention: {name} must be an int32 tensor on {like.device}")
-    if tuple(t.shape) not in shapes or (t.dim() and t.stride(-1) != 1):
+    if t.shape not in shapes or t.stride(-1) != 1:
         raise ValueError(f"masked_attention: {name} has shape {tuple(t.shape)} (contiguous {shapes} expected)")
 
 
@@ -783,14 +815,15 @@ def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=No
     * ``softcap``: cap of the scores;  ``slopes`` fp32 [H]: linear bias by distance
 
     GPU: bf16 / fp16, D % 8 == 0, D <= 256 (csrc/masked_attention.hip).  Inference only."""
-    if q.dim() != 4 or k.dim() != 4 or tuple(k.shape) != tuple(v.shape):
-        raise ValueError(f"masked_attention: q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
-    B, Nq, H, D = q.shape
-    if k.shape[0] != B or k.shape[3] != D or k.shape[2] < 1 or H % k.shape[2] or D < 1:
-        raise ValueError(f"masked_attention: q {tuple(q.shape)} does not go with k / v {tuple(k.shape)}")
-    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+    qs, ks, dtype, device = q.shape, k.shape, q.dtype, q.device
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape:
+        raise ValueError(f"masked_attention: q {tuple(qs)} k {tuple(ks)} v {tuple(v.shape)}")
+    B, Nq, H, D = qs
+    if ks[0] != B or ks[3] != D or ks[2] < 1 or H % ks[2] or D < 1:
+        raise ValueError(f"masked_attention: q {tuple(qs)} does not go with k / v {tuple(ks)}")
+    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
         raise TypeError("masked_attention: q, k and v must share dtype and device")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("masked_attention: inference only (no gradients)")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not math.isfinite(scale):
@@ -816,10 +849,9 @@ def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=No
             raise ValueError("masked_attention: prefix needs causal=True")
         _index_arg("prefix", prefix, q, [(B,)] if documents is None else [(n,), (B, n)])
     if slopes is not None and (not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32
-                               or slopes.device != q.device or tuple(slopes.shape) != (H,)
-                               or not slopes.is_contiguous()):
-        raise ValueError(f"masked_attention: slopes must be contiguous fp32 [{H}] on {q.device}")
-    if Nq >= 2 ** 31 or k.shape[1] >= 2 ** 31:
+                               or slopes.device != device or slopes.shape != (H,) or not slopes.is_contiguous()):
+        raise ValueError(f"masked_attention: slopes must be contiguous fp32 [{H}] on {device}")
+    if Nq >= 2 ** 31 or ks[1] >= 2 ** 31:
         raise ValueError("masked_attention: more than 2^31 - 1 queries or keys")
     args = (q, k, v, scale, bool(causal), q_start, lengths, prefix, documents, softcap, slopes)
     return _lib.masked_attention(*args, _canon_batch(B)) if _hip(q) else ref.masked_attention(*args)

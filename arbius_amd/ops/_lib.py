@@ -8,7 +8,9 @@ shared GPU box can fault the whole node).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -92,9 +94,10 @@ _SIGS = {
     "arb_set_h264_sync": (None, [c_int]),
     "arb_quantize_rows": (c_int, [c_void_p, c_long, c_void_p, c_void_p, c_float, c_void_p, c_int, c_void_p, c_long,
                                   c_int, c_int, c_void_p]),
-    "arb_linear_int8": (c_int, [c_void_p, c_long, c_void_p, c_void_p, c_long] + [c_void_p] * 4 + [c_int] * 5
-                        + [c_void_p]),
-    "arb_masked_attention": (c_int, [c_void_p] * 12 + [c_float, c_float, c_int, c_void_p]),
+    "arb_linear_int8": (c_int, [c_void_p, c_long] + [c_void_p] * 3 + [c_float] + [c_void_p] * 2 + [c_long]
+                        + [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
+    "arb_masked_attention": (c_int, [c_void_p] * 4 + [ctypes.c_char_p] + [c_void_p] * 6 + [c_float, c_float, c_int,
+                                                                                          c_void_p]),
     "arb_masked_attention_workspace": (c_size_t, [c_int, c_long] + [c_int] * 5),
 }
 
@@ -1116,23 +1119,15 @@ def _el(op, t):
         raise TypeError(f"{op}: the HIP kernel takes bf16 or fp16 tensors, got {t.dtype}") from None
 
 
-class _on:
-    """Launch on ``t``'s device and its current stream, whatever the caller's current device is."""
-    __slots__ = ("guard",)
-
-    def __init__(self, t):
-        dev = t.device
-        same = _AUDIT is not None or dev.index is None or dev.index == torch.cuda.current_device()
-        self.guard = None if same else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return _stream()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(t, fn, *args):
+    """fn(*args, stream) on ``t``'s device and its current stream, whatever the caller's current device is."""
+    if _AUDIT is not None:
+        return fn(*args, 0)
+    idx = t.device.index
+    if idx == torch.cuda.current_device():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    with torch.cuda.device(idx):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(idx))
 
 
 def _rows2d(x):
@@ -1154,9 +1149,8 @@ def quantize_rows(x, norm=None):
     scale = torch.empty(R, dtype=torch.float32, device=x.device)
     gamma, beta, eps = norm if norm is not None else (None, None, 0.0)
     if R:
-        with _on(x) as stream:
-            _check(_fn("arb_quantize_rows")(_p(x2), x2.stride(0), _p(gamma), _p(beta), float(eps), _p(q), ldq,
-                                            _p(scale), R, K, el, stream), "quantize_rows")
+        _check(_launch(x, _fn("arb_quantize_rows"), _p(x2), x2.stride(0), _p(gamma), _p(beta), float(eps), _p(q), ldq,
+                       _p(scale), R, K, el), "quantize_rows")
     return (q if ldq == K else q[:, :K]), scale
 
 
@@ -1165,15 +1159,38 @@ _INT8_ACT = {None: 0, "gelu": 1, "quick_gelu": 2, "geglu": 3}
 
 def linear_int8(q, sx, w, sw, b, residual, act, shape, dtype):
     """q [M, K] / w [N, K] int8 rows with fp32 scales -> act(sx sw (q . w) + b + residual) [*shape, N]."""
-    el = _EL[dtype]
-    M, K = q.shape
-    N = w.shape[0]
-    y = torch.empty(*shape, N // 2 if act == "geglu" else N, dtype=dtype, device=q.device)
-    audit_note("linear_int8", M=M, N=N, K=K)
-    if y.numel():
-        with _on(q) as stream:
-            _check(_fn("arb_linear_int8")(_p(q), q.stride(0), _p(sx), _p(w), w.stride(0), _p(sw), _p(b), _p(residual),
-                                          _p(y), M, N, K, _INT8_ACT[act], el, stream), "linear_int8")
+    return _linear_int8(q, sx, None, w, sw, b, residual, act, shape, dtype)
+
+
+def linear_int8_of(x, norm, w, sw, b, residual, act):
+    """``linear_int8`` of the quantised rows of x [..., K] (norm = (gamma, beta, eps): of LayerNorm(x)), their int8
+    form in a workspace of the call."""
+    return _linear_int8(x, None, norm, w, sw, b, residual, act, x.shape[:-1], x.dtype)
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _linear_int8(x, sx, norm, w, sw, b, residual, act, shape, dtype):
+    el = _EL.get(dtype)
+    if el is None:
+        raise TypeError(f"linear_int8: the HIP kernel takes bf16 or fp16 tensors, got {dtype}")
+    N, K = w.shape
+    x2 = x if sx is not None else _rows2d(x)
+    M, ldx = x2.shape[0], x2.stride(0)
+    y = torch.empty((*shape, N // 2 if act == "geglu" else N), dtype=dtype, device=w.device)
+    if _AUDIT is not None:
+        audit_note("linear_int8", M=M, N=N, K=K)
+    if not M or not N:
+        return y
+    ws = None
+    if sx is None:                 # int8 rows of a multiple of 16 bytes, then the scales
+        ws = torch.empty(M * ((K + 15) // 16 * 16 + 4), dtype=torch.uint8, device=w.device)
+    gamma, beta, eps = norm if norm is not None else (None, None, 0.0)
+    _check(_launch(w, _fn("arb_linear_int8"), x2.data_ptr(), ldx, _ptr(sx), _ptr(gamma), _ptr(beta), eps, _ptr(ws),
+                   w.data_ptr(), w.stride(0), sw.data_ptr(), _ptr(b), _ptr(residual), y.data_ptr(), M, N, K,
+                   _INT8_ACT[act], el), "linear_int8")
     return y
 
 
@@ -1186,7 +1203,8 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
     if D % 8 or D > 256:
         raise ValueError(f"masked_attention: D={D} not a multiple of 8 up to 256")
     for t in (q, k, v):
-        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+        sb, sn, sh, sd = t.stride()
+        if sd != 1 or (sb | sn | sh) % 8 or t.data_ptr() % 16:
             raise ValueError("masked_attention: last dim must be contiguous, strides/base 16B aligned")
     # keys that share memory (a token stride below D) or lie 16 MiB apart are out of the tile loads' addressing
     k, v = (t if D <= t.stride(1) < 1 << 23 else t.contiguous() for t in (k, v))
@@ -1198,14 +1216,21 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
     starts = isinstance(q_start, torch.Tensor)
     docs_sb = documents.stride(0) if documents is not None and documents.dim() == 2 else 0
     prefix_sb = 0 if prefix is None else prefix.stride(0) if documents is None or prefix.dim() == 2 else 0
-    strides = (c_long * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
     plan_b = plan_b or B
-    ints = (c_long * 12)(B, H, Hkv, Nq, Nk, D, int(causal), 0 if starts else q_start,
-                         0 if documents is None else documents.shape[-1] - 1, docs_sb, prefix_sb, plan_b)
-    wsb = _fn("arb_masked_attention_workspace")(B, plan_b, H, Hkv, Nq, Nk, D)
+    wsb = _masked_workspace(B, plan_b, H, Hkv, Nq, Nk, D)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
-    with _on(q) as stream:
-        _check(_fn("arb_masked_attention")(_p(q), _p(k), _p(v), _p(o), strides, ints, _p(q_start if starts else None),
-                                           _p(lengths), _p(documents), _p(prefix), _p(slopes), _p(ws), float(scale),
-                                           float(softcap or 0.0), el, stream), "masked_attention")
+    ints = _MASKED_INTS.pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3], B, H, Hkv, Nq, Nk, D,
+                             causal, 0 if starts else q_start, 0 if documents is None else documents.shape[-1] - 1,
+                             docs_sb, prefix_sb, plan_b)
+    _check(_launch(q, _fn("arb_masked_attention"), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ints,
+                   _ptr(q_start if starts else None), _ptr(lengths), _ptr(documents), _ptr(prefix), _ptr(slopes),
+                   _ptr(ws), scale, softcap or 0.0, el), "masked_attention")
     return o
+
+
+_MASKED_INTS = struct.Struct("=24q")
+
+
+@functools.lru_cache(maxsize=4096)
+def _masked_workspace(*shape):
+    return _fn("arb_masked_attention_workspace")(*shape)

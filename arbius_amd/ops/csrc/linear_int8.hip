@@ -22,10 +22,15 @@ __device__ __forceinline__ uint32_t enc16(float f) {
   else return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
-__device__ __forceinline__ float act_f(float y, int act) {
-  if (act == ACT_GELU) return gelu_f(y);
-  if (act == ACT_QUICK_GELU) return y * __builtin_amdgcn_rcpf(1.f + fast_exp(-1.702f * y));
-  return y;
+// the activation of 8 values (uniform branch outside the loop)
+__device__ __forceinline__ void act8(float (&y)[8], int act) {
+  if (act == ACT_GELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = gelu_f(y[e]);
+  } else if (act == ACT_QUICK_GELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] *= __builtin_amdgcn_rcpf(1.f + fast_exp(-1.702f * y[e]));
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -201,6 +206,7 @@ struct LinArgs {
   uint16_t* y;           // [M, N] (N / 2 for geglu)
   long ldx, ldw;
   int M, N, K, act;
+  bool vec;              // 16-byte accesses to y and res: N (N / 2) % 8 == 0, res aligned
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -211,11 +217,12 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ i32x16 mma_i8(uint4 a, uint4 b, i32x16 c) {
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
-// 16 bytes per lane straight into LDS (lane-linear from the wave-uniform lds) through a buffer resource over
-// [base, base + nbytes): a lane whose offset lies past it writes zeros.
-__device__ __forceinline__ void dma_i8(const int8_t* base, int nbytes, void* lds, unsigned off) {
-  __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, nbytes, 0x00020000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, 0, 0, 0);
+// 16 bytes per lane from base + off + k0 straight into LDS (lane-linear from the wave-uniform lds); a lane with
+// off = kZeros writes zeros.  base and k0 are uniform: a load costs its own instruction and the LDS address.
+constexpr unsigned kZeros = 0x80000000u;
+__device__ __forceinline__ void dma_i8(const int8_t* base, void* lds, unsigned off, int k0) {
+  __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, 0x7fffffff, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, k0, 0, 0);
 }
 template <int N>
 __device__ __forceinline__ void wait_dma() {                      // at most N of this wave's loads still in flight
@@ -225,135 +232,239 @@ template <int V>
 struct Stage {
   static constexpr int value = V;
 };
+template <int S>
+__device__ __forceinline__ int8_t* ring_of(int8_t* r0, int8_t* r1, int8_t* r2, int8_t* r3) {
+  if constexpr (S == 0) return r0;
+  else if constexpr (S == 1) return r1;
+  else if constexpr (S == 2) return r2;
+  else return r3;
+}
 
-// Epilogue of one 32 (tokens) x 32 W (channels) strip of a wave: the fp32 results cross a wave-private LDS patch
-// (a lane holds 4 channels of one token; the stores want runs of channels), then residual, activation
-// and one rounding to the output type; 16 bytes per lane where N allows it.
-template <int EL, int W>
-__device__ __forceinline__ void store_strip(const LinArgs& p, const float* patch, int m0, int n0, int NO, int act) {
-  constexpr int LD = 32 * W + 4;
-  const int lane = threadIdx.x & 63;
-  auto finish = [&](float y, long at) {
-    if (p.res) y += dec16<EL>(p.res[at]);
-    return act_f(y, act);
-  };
-  if (NO % 8 == 0) {
-    constexpr int LPR = 4 * W;                                    // lanes per row, 8 channels each
+// Scales and biases of a workgroup's tile.  They are read before the K loop (one row and one channel per thread, in
+// registers meanwhile) and reach LDS after it: the epilogue waits for no memory.
+template <int BM, int BN>
+struct TileScales {
+  float sx[BM], sw[BN], bias[BN];
+};
+template <int EL, int BM, int BN, int NT>
+struct ScaleRegs {
+  static constexpr int NX = (BM + NT - 1) / NT, NWR = (BN + NT - 1) / NT;
+  float sx[NX], sw[NWR];
+  uint16_t bias[NWR];
+  // row(r): the weight row of row r of the W tile, -1 past the last one
+  template <typename F>
+  __device__ __forceinline__ void load(const LinArgs& p, int m0, F row) {
 #pragma unroll
-    for (int it = 0; it < 32 * LPR / 64; ++it) {
-      const int r = (it * 64 + lane) / LPR, c = (it * 64 + lane) % LPR * 8;
-      if (m0 + r >= p.M || n0 + c >= NO) continue;
-      const long at = (long)(m0 + r) * NO + n0 + c;
-      float f[8];
-      *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(patch + r * LD + c);
-      *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(patch + r * LD + c + 4);
-      if (p.res) {
-        float g[8];
-        dec8<EL>(ld16(p.res + at), g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] += g[e];
-      }
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = enc16<EL>(act_f(f[2 * e], act)) | (enc16<EL>(act_f(f[2 * e + 1], act)) << 16);
-      st16(p.y + at, make_uint4(w[0], w[1], w[2], w[3]));
+    for (int i = 0; i < NX; ++i) {
+      const int m = m0 + (int)threadIdx.x + NT * i;
+      sx[i] = p.sx[min(m, p.M - 1)];
     }
-  } else {
-    for (int e = lane; e < 32 * 32 * W; e += 64) {
-      const int r = e / (32 * W), c = e % (32 * W);
-      if (m0 + r >= p.M || n0 + c >= NO) continue;
-      const long at = (long)(m0 + r) * NO + n0 + c;
-      p.y[at] = (uint16_t)enc16<EL>(finish(patch[r * LD + c], at));
+#pragma unroll
+    for (int i = 0; i < NWR; ++i) {
+      const int n = max(0, row(min((int)threadIdx.x + NT * i, BN - 1)));
+      sw[i] = p.sw[n];
+      bias[i] = p.b ? p.b[n] : 0;
     }
   }
+  __device__ __forceinline__ void store(TileScales<BM, BN>& t) const {
+#pragma unroll
+    for (int i = 0; i < NX; ++i)
+      if ((int)threadIdx.x + NT * i < BM) t.sx[threadIdx.x + NT * i] = sx[i];
+#pragma unroll
+    for (int i = 0; i < NWR; ++i)
+      if ((int)threadIdx.x + NT * i < BN) {
+        t.sw[threadIdx.x + NT * i] = sw[i];
+        t.bias[threadIdx.x + NT * i] = dec16<EL>(bias[i]);
+      }
+  }
+};
+
+// Two floats as two 16-bit values, rounded to nearest even (one instruction each pair)
+template <int EL>
+__device__ __forceinline__ uint32_t enc16x2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (EL == 0) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+  }
+}
+
+// A lane's 8 channels (GLU: and their gates), the same for every token it finishes.
+template <bool GLU>
+struct Lane8 {
+  float sw[8], bias[8], gsw[GLU ? 8 : 1], gbias[GLU ? 8 : 1];
+  template <int GATE>
+  __device__ __forceinline__ void read(const float* s, const float* b) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sw[e] = s[e];
+      bias[e] = b[e];
+      if constexpr (GLU) {
+        gsw[e] = s[GATE + e];
+        gbias[e] = b[GATE + e];
+      }
+    }
+  }
+};
+
+// Channels n .. + 7 of token m: the KW partial sums of the patches, scales, bias, residual, activation, one
+// rounding.  off: the values' place in a patch, their gates (GLU) GATE further on.
+template <int EL, bool GLU, int KW, int GATE, bool VEC>
+__device__ __forceinline__ void finish8(const LinArgs& p, const int* const (&patch)[KW], int off, float sx,
+                                        const Lane8<GLU>& ch, int m, int n, int NO) {
+  const uint16_t* __restrict__ res = p.res;
+  uint16_t* __restrict__ y = p.y;
+  auto sums = [&](int at, float (&f)[8]) {
+    int t[8];
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      const int4 u = *reinterpret_cast<const int4*>(patch[w] + off + at);
+      const int4 v = *reinterpret_cast<const int4*>(patch[w] + off + at + 4);
+      const int uv[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = w ? t[e] + uv[e] : uv[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (float)t[e] * sx;
+  };
+  float f[8];
+  sums(0, f);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = fmaf(f[e], ch.sw[e], ch.bias[e]);
+  if constexpr (GLU) {
+    float g[8];
+    sums(GATE, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= gelu_f(fmaf(g[e], ch.gsw[e], ch.gbias[e]));
+  }
+  if (m >= p.M) return;
+  const long at = (long)m * NO + n;
+  if constexpr (VEC) {
+    if (n >= NO) return;
+    if (res) {
+      float g[8];
+      dec8<EL>(ld16(res + at), g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] += g[e];
+    }
+    if constexpr (!GLU) act8(f, p.act);
+    st16(y + at, make_uint4(enc16x2<EL>(f[0], f[1]), enc16x2<EL>(f[2], f[3]), enc16x2<EL>(f[4], f[5]),
+                            enc16x2<EL>(f[6], f[7])));
+  } else {
+    if (res) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < NO) f[e] += dec16<EL>(res[at + e]);
+    }
+    if constexpr (!GLU) act8(f, p.act);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (n + e < NO) y[at + e] = (uint16_t)enc16<EL>(f[e]);
+  }
+}
+
+// Tile of workgroup `lin`: XCD-contiguous, in groups of 8 token tiles x all channel tiles (token tile fastest), so
+// the tiles in flight on an XCD share rows of both operands in its L2.
+__device__ __forceinline__ void tile_of(int mt, int nt, int& m, int& n) {
+  const int lin = xcd_remap(blockIdx.x, mt * nt);
+  const int grp = lin / (8 * nt), in = lin - grp * 8 * nt, gm = min(8, mt - 8 * grp);
+  m = 8 * grp + in % gm;
+  n = in / gm;
+}
+
+// A strip of 32 tokens x 32 TN weight rows as integers into a patch [32][32 TN + 4].
+template <int TM, int TN>
+__device__ __forceinline__ void put_strip(const i32x16 (&acc)[TN][TM], int b, int* patch) {
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int a = 0; a < TN; ++a)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const i32x16& x = acc[a][b];
+      *reinterpret_cast<int4*>(patch + col * (32 * TN + 4) + 32 * a + 2 * i + 4 * half) =
+          make_int4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    }
 }
 
 // BM tokens x BN weight rows per workgroup, WM x WN waves, K in tiles of 128 bytes: both operands go straight to
 // LDS (ring of NS stages, NS - 1 tiles in flight, counted waits, one barrier per tile), chunks XOR-swizzled
 // by the row on the source address so that fragment reads touch every bank once.  W is the A operand: a
-// lane's accumulators are 4 consecutive channels of one token.
+// lane's accumulators are 4 consecutive channels of one token; the epilogue takes them through an LDS
+// patch, so that a lane stores (and loads residuals) 8 channels wide with their scales in registers.
 // GLU: 32-row groups of the W tile alternate value rows and gate rows of the same channels, so both
 // halves of an output meet in one lane.
 template <int EL, bool GLU, int BM, int BN, int WM, int WN, int NS>
 __global__ void __launch_bounds__(64 * WM * WN, 1) linear_int8_kernel(LinArgs p) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int PRE = TM + TN <= 3 ? 4 : TM + TN <= 4 ? 2 : 1;    // K steps whose fragments are read together
   constexpr int XCH = BM / 8 / NW, WCH = BN / 8 / NW;             // DMA instructions per wave and tile (8 rows each)
   constexpr int LPT = XCH + WCH, STAGE = (BM + BN) * 128;
-  constexpr int PW = GLU ? TN / 2 : TN;                           // 32-channel groups a wave puts out
   static_assert(XCH * 8 * NW == BM && WCH * 8 * NW == BN && (!GLU || TN % 2 == 0), "tile shape");
-  static_assert(32 * (32 * PW + 4) * 4 * NW <= NS * STAGE, "patches fit the ring");
-  __shared__ __attribute__((aligned(16))) int8_t ring[NS][STAGE];
+  constexpr int LD = 32 * TN + 4, PATCH = 32 * LD;                // a wave's epilogue patch (ints)
+  static_assert(PATCH * 4 * (NW / 2) <= STAGE, "half of the patches fit a ring stage");
+  __shared__ TileScales<BM, BN> scales;
+  // one __shared__ object per stage, each reached through compile-time stage numbers only: hipcc then knows that
+  // reads of one stage do not depend on the loads into the others, and leaves those in flight
+  __shared__ __attribute__((aligned(16))) int8_t ring0[STAGE];
+  __shared__ __attribute__((aligned(16))) int8_t ring1[STAGE];
+  __shared__ __attribute__((aligned(16))) int8_t ring2[NS > 2 ? STAGE : 16];
+  __shared__ __attribute__((aligned(16))) int8_t ring3[NS > 3 ? STAGE : 16];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, col = lane & 31, half = lane >> 5;
   const int NO = GLU ? p.N / 2 : p.N;                             // output channels
   constexpr int BO = GLU ? BN / 2 : BN;                           // ... per workgroup
-  // tile order: XCD-contiguous, in groups of 8 token tiles x all channel tiles (token tile fastest), so the
-  // tiles in flight on an XCD share rows of both operands in its L2
-  const int mt = (p.M + BM - 1) / BM, nt = (NO + BO - 1) / BO;
-  const int lin = xcd_remap(blockIdx.x, mt * nt);
-  const int grp = lin / (8 * nt), in = lin - grp * 8 * nt, gm = min(8, mt - 8 * grp);
-  const int m0 = (8 * grp + in % gm) * BM, n0 = in / gm * BO;
+  int m0, n0;
+  tile_of((p.M + BM - 1) / BM, (NO + BO - 1) / BO, m0, n0);
+  m0 *= BM;
+  n0 *= BO;
+  ScaleRegs<EL, BM, BN, 64 * NW> sr;
+  sr.load(p, m0, [&](int r) {
+    const int n = GLU ? n0 + (r >> 6) * 32 + (r & 31) : n0 + r;
+    return n >= NO ? -1 : GLU && ((r >> 5) & 1) ? NO + n : n;
+  });
 
   const int kp = (p.K + 15) & ~15;                                // bytes of a row that are loaded
   const int nk = (kp + 127) / 128;
   const int8_t* xb = p.x + (long)m0 * p.ldx;
-  const int8_t* wb = GLU ? p.w : p.w + (long)n0 * p.ldw;
-  const int xbytes = (int)min((long)min(BM, p.M - m0) * p.ldx, 0x7fffffffL);
-  constexpr unsigned OOB = 0x80000000u;
-  unsigned xo[XCH];
-  int kc[XCH > WCH ? XCH : WCH];                                  // byte of the row a DMA lane starts at
-#pragma unroll
-  for (int i = 0; i < XCH; ++i) {
-    const int r = 8 * (wave + NW * i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-    xo[i] = m0 + r < p.M ? (unsigned)(r * (int)p.ldx + 16 * c) : OOB;
-  }
-  // W rows: 64-bit row starts for GLU (two far row groups), offsets in the tile otherwise
-  unsigned wo[WCH];
-  const int8_t* wrow[GLU ? WCH : 1];
-#pragma unroll
-  for (int i = 0; i < WCH; ++i) {
-    const int r = 8 * (wave + NW * i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-    if constexpr (GLU) {
-      const int n = n0 + (r >> 6) * 32 + (r & 31);
-      wo[i] = n < NO ? 16 * c : OOB;
-      wrow[i] = nullptr;
-    } else {
-      wo[i] = n0 + r < NO ? (unsigned)(r * (int)p.ldw + 16 * c) : OOB;
-    }
-  }
+  unsigned xo[XCH], wo[WCH];
+  const int8_t* wb[WCH];                                          // uniform: an instruction's 8 rows are of one kind
+  int kc[XCH > WCH ? XCH : WCH];                                  // byte of the K tile a lane starts at
 #pragma unroll
   for (int i = 0; i < (XCH > WCH ? XCH : WCH); ++i) {
     const int r = 8 * (wave + NW * i) + (lane >> 3);
     kc[i] = 16 * ((lane & 7) ^ ((r >> 1) & 7));
   }
-  (void)wrow;
+#pragma unroll
+  for (int i = 0; i < XCH; ++i) {
+    const int r = 8 * (wave + NW * i) + (lane >> 3);
+    xo[i] = m0 + r < p.M ? (unsigned)(r * (int)p.ldx + kc[i]) : kZeros;
+  }
+#pragma unroll
+  for (int i = 0; i < WCH; ++i) {
+    const int r0 = 8 * (wave + NW * i), r = r0 + (lane >> 3);
+    const int row = GLU ? (r >> 6) * 32 + (r & 31) : r;           // of the tile's value rows / gate rows
+    wb[i] = p.w + ((GLU && ((r0 >> 5) & 1) ? NO : 0) + (long)n0) * p.ldw;
+    wo[i] = n0 + row < NO ? (unsigned)(row * (int)p.ldw + kc[i]) : kZeros;
+  }
   auto issue = [&](auto stage, int kt) __attribute__((always_inline)) {
-    int8_t* dst = ring[decltype(stage)::value];
+    int8_t* dst = ring_of<decltype(stage)::value>(ring0, ring1, ring2, ring3);
     const int k0 = 128 * kt;
-    const bool tail = k0 + 128 > kp;
+    if (k0 + 128 <= kp) {
 #pragma unroll
-    for (int i = 0; i < XCH; ++i) {
-      unsigned off = xo[i];
-      if (tail && k0 + kc[i] >= kp) off = OOB;
-      dma_i8(xb + k0, xbytes - k0, dst + 1024 * (wave + NW * i), off);
-    }
+      for (int i = 0; i < XCH; ++i) dma_i8(xb, dst + 1024 * (wave + NW * i), xo[i], k0);
 #pragma unroll
-    for (int i = 0; i < WCH; ++i) {
-      unsigned off = wo[i];
-      if (tail && k0 + kc[i] >= kp) off = OOB;
-      if constexpr (GLU) {
-        // the 8 rows of one DMA instruction lie in one group: a uniform base, rows ldw apart
-        const int r = 8 * (wave + NW * i), n = n0 + (r >> 6) * 32 + (r & 31);
-        const int8_t* base = p.w + (long)((r >> 5) & 1 ? NO + n : n) * p.ldw + k0;
-        const int left = min(8, NO - n);
-        if (off != OOB) off += (unsigned)((lane >> 3) * (int)p.ldw);
-        dma_i8(base, left > 0 ? left * (int)p.ldw - k0 : 0, dst + BM * 128 + 1024 * (wave + NW * i), off);
-      } else {
-        dma_i8(wb + k0, (int)min((long)min(BN, NO - n0) * p.ldw, 0x7fffffffL) - k0,
-               dst + BM * 128 + 1024 * (wave + NW * i), off);
-      }
+      for (int i = 0; i < WCH; ++i) dma_i8(wb[i], dst + BM * 128 + 1024 * (wave + NW * i), wo[i], k0);
+    } else {                                                      // the row ends inside the tile
+#pragma unroll
+      for (int i = 0; i < XCH; ++i)
+        dma_i8(xb, dst + 1024 * (wave + NW * i), k0 + kc[i] < kp ? xo[i] : kZeros, k0);
+#pragma unroll
+      for (int i = 0; i < WCH; ++i)
+        dma_i8(wb[i], dst + BM * 128 + 1024 * (wave + NW * i), k0 + kc[i] < kp ? wo[i] : kZeros, k0);
     }
   };
 
@@ -369,20 +480,35 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) linear_int8_kernel(LinArgs p)
     else wait_dma<0>();
     __builtin_amdgcn_s_barrier();                                 // tile kt is in LDS for every wave
     if (kt + NS - 1 < nk) issue(Stage<(S + NS - 1) % NS>(), kt + NS - 1);   // that stage was read at kt - 1
-    const int8_t* sx = ring[S] + wm * (BM / WM) * 128;
-    const int8_t* sw = ring[S] + (BM + wn * (BN / WN)) * 128;
+    const int8_t* st = ring_of<S>(ring0, ring1, ring2, ring3);
+    const int8_t* sx = st + wm * (BM / WM) * 128;
+    const int8_t* sw = st + (BM + wn * (BN / WN)) * 128;
+    // Fragments are read PRE steps of 32 at a time, all before the products that use them (left to itself hipcc
+    // puts every read right in front of its product and waits out the LDS latency four times a tile).
+    uint4 af[2][PRE][TN], bf[2][PRE][TM];
+    auto read = [&](int k) __attribute__((always_inline)) {
+      const int at = 128 * col + 16 * ((2 * k + half) ^ ((col >> 1) & 7));
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const int at = 128 * col + 16 * ((2 * ks + half) ^ ((col >> 1) & 7));
-      uint4 af[TN], bf[TM];
+      for (int a = 0; a < TN; ++a) af[k / PRE & 1][k % PRE][a] = ld16(sw + 4096 * a + at);
 #pragma unroll
-      for (int a = 0; a < TN; ++a) af[a] = ld16(sw + 4096 * a + at);
+      for (int b = 0; b < TM; ++b) bf[k / PRE & 1][k % PRE][b] = ld16(sx + 4096 * b + at);
+    };
 #pragma unroll
-      for (int b = 0; b < TM; ++b) bf[b] = ld16(sx + 4096 * b + at);
+    for (int k = 0; k < PRE; ++k) read(k);
 #pragma unroll
-      for (int a = 0; a < TN; ++a)
+    for (int g = 0; g < 4 / PRE; ++g) {
+      if (g + 1 < 4 / PRE) {
 #pragma unroll
-        for (int b = 0; b < TM; ++b) acc[a][b] = mma_i8(af[a], bf[b], acc[a][b]);
+        for (int k = 0; k < PRE; ++k) read((g + 1) * PRE + k);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < PRE; ++k)
+#pragma unroll
+        for (int a = 0; a < TN; ++a)
+#pragma unroll
+          for (int b = 0; b < TM; ++b) acc[a][b] = mma_i8(af[g & 1][k][a], bf[g & 1][k][b], acc[a][b]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   issue(Stage<0>(), 0);
@@ -398,34 +524,129 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) linear_int8_kernel(LinArgs p)
       if (kt + 3 < nk) step(Stage<3 % NS>(), kt + 3);
     }
   }
+  sr.store(scales);
   __syncthreads();                                                // the ring becomes the waves' patches
 
-  float* patch = reinterpret_cast<float*>(&ring[0][0]) + wave * 32 * (32 * PW + 4);
-  const int nw = n0 + wn * 32 * PW;                               // this wave's first output channel
+  int* patch = reinterpret_cast<int*>(wave < NW / 2 ? ring0 : ring1) + wave % (NW / 2) * PATCH;
+  const int* const patches[1] = {patch};
+  constexpr int OW = GLU ? 16 * TN : 32 * TN, LPR = OW / 8, RPI = 64 / LPR;   // channels of a strip, lanes, rows
+  const int c = lane % LPR * 8, pc = GLU ? c / 32 * 64 + c % 32 : c, n = n0 + wn * OW + c;
+  Lane8<GLU> ch;
+  ch.template read<32>(scales.sw + wn * 32 * TN + pc, scales.bias + wn * 32 * TN + pc);
+  auto strips = [&](auto vec) __attribute__((always_inline)) {
 #pragma unroll
-  for (int b = 0; b < TM; ++b) {
-    const int m = m0 + wm * (BM / WM) + 32 * b;
-    const float sx = m + col < p.M ? p.sx[m + col] : 0.f;
+    for (int b = 0; b < TM; ++b) {
+      put_strip<TM, TN>(acc, b, patch);
 #pragma unroll
-    for (int g = 0; g < PW; ++g)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int c = 32 * g + 2 * i + 4 * half;
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = min(nw + c + e, NO - 1);                  // channels past the last one are not stored
-          y[e] = (float)acc[GLU ? 2 * g : g][b][i + e] * sx * p.sw[n];
-          if (p.b) y[e] += dec16<EL>(p.b[n]);
-          if constexpr (GLU) {
-            float gate = (float)acc[2 * g + 1][b][i + e] * sx * p.sw[NO + n];
-            if (p.b) gate += dec16<EL>(p.b[NO + n]);
-            y[e] *= gelu_f(gate);
-          }
-        }
-        *reinterpret_cast<float4*>(patch + col * (32 * PW + 4) + c) = make_float4(y[0], y[1], y[2], y[3]);
+      for (int it = 0; it < 32 / RPI; ++it) {
+        const int r = it * RPI + lane / LPR, mr = wm * (BM / WM) + 32 * b + r;
+        finish8<EL, GLU, 1, 32, decltype(vec)::value != 0>(p, patches, r * LD + pc, scales.sx[mr], ch, m0 + mr, n, NO);
       }
-    store_strip<EL, PW>(p, patch, m, nw, NO, GLU ? ACT_NONE : p.act);
+    }
+  };
+  if (p.vec) strips(Stage<1>());
+  else strips(Stage<0>());
+}
+
+__device__ __forceinline__ uint4 load_i8(const int8_t* base, unsigned off, int k0) {
+  __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, 0x7fffffff, 0x00020000);
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, k0, 0));
+}
+
+// Few tokens: 16 TM tokens x 16 TN weight rows per workgroup, and its KW waves split K.  No LDS and no barrier in the
+// loop: each wave keeps two K tiles of 128 bytes of both operands in flight in its own registers, a lane's
+// 16 bytes being its 16x16x64 MFMA fragment as it lies in memory.  The integer partial sums of the waves meet
+// in LDS.  Bound by the read of the weight: 1 x 2048 -> 8192 in 6.2 us, 2.7 TB/s.
+template <int EL, bool GLU, int TM, int TN, int KW>
+__global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs p) {
+  constexpr int BM = 16 * TM, BN = 16 * TN, BO = GLU ? BN / 2 : BN, LD = BN + 4;
+  static_assert(!GLU || TN % 2 == 0, "value and gate groups");
+  __shared__ __attribute__((aligned(16))) int patch[KW][BM * LD];
+  __shared__ TileScales<BM, BN> scales;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int NO = GLU ? p.N / 2 : p.N;
+  int m0, n0;
+  tile_of((p.M + BM - 1) / BM, (NO + BO - 1) / BO, m0, n0);
+  m0 *= BM;
+  n0 *= BO;
+  // rows past the last one repeat it: their results are not stored.  GLU: 16-row groups alternate values and gates
+  unsigned xo[TM], wo[TN];
+#pragma unroll
+  for (int b = 0; b < TM; ++b) xo[b] = (unsigned)(min(16 * b + r16, p.M - 1 - m0) * (int)p.ldx + 16 * g);
+#pragma unroll
+  for (int a = 0; a < TN; ++a) {
+    const int r = GLU ? 16 * (a >> 1) + r16 : 16 * a + r16;
+    wo[a] = (unsigned)(min(r, NO - 1 - n0) * (int)p.ldw + 16 * g);
+  }
+  ScaleRegs<EL, BM, BN, 64 * KW> sr;
+  sr.load(p, m0, [&](int r) {
+    const int n = GLU ? n0 + (r >> 5) * 16 + (r & 15) : n0 + r;
+    return n >= NO ? -1 : GLU && ((r >> 4) & 1) ? NO + n : n;
+  });
+  const int kp = (p.K + 15) & ~15, nk = (kp + 127) / 128;
+  const int8_t* xb = p.x + (long)m0 * p.ldx;
+  const int8_t* wb = p.w + (long)n0 * p.ldw;
+  const int8_t* gb = GLU ? wb + (long)NO * p.ldw : wb;
+
+  uint4 xf[2][2][TM], wf[2][2][TN];
+  auto load = [&](auto buf, int kt) __attribute__((always_inline)) {
+    constexpr int B = decltype(buf)::value;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int k0 = 128 * kt + 64 * s;
+      const unsigned past = k0 + 16 * g < kp ? 0u : kZeros;       // chunks behind the row
+#pragma unroll
+      for (int a = 0; a < TN; ++a)
+        wf[B][s][a] = load_i8(GLU && (a & 1) ? gb : wb, wo[a] | past, k0);
+#pragma unroll
+      for (int b = 0; b < TM; ++b) xf[B][s][b] = load_i8(xb, xo[b] | past, k0);
+    }
+  };
+  i32x4 acc[TN][TM];
+#pragma unroll
+  for (int a = 0; a < TN; ++a)
+#pragma unroll
+    for (int b = 0; b < TM; ++b) acc[a][b] = (i32x4){};
+  auto mma = [&](auto buf) __attribute__((always_inline)) {
+    constexpr int B = decltype(buf)::value;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int a = 0; a < TN; ++a)
+#pragma unroll
+        for (int b = 0; b < TM; ++b)
+          acc[a][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[B][s][a]),
+                                                            __builtin_bit_cast(i32x4, xf[B][s][b]), acc[a][b], 0, 0, 0);
+  };
+  if (wave < nk) load(Stage<0>(), wave);
+  if (wave + KW < nk) load(Stage<1>(), wave + KW);
+  for (int kt = wave; kt < nk; kt += 2 * KW) {
+    mma(Stage<0>());
+    if (kt + 2 * KW < nk) load(Stage<0>(), kt + 2 * KW);
+    if (kt + KW < nk) {
+      mma(Stage<1>());
+      if (kt + 3 * KW < nk) load(Stage<1>(), kt + 3 * KW);
+    }
+  }
+  // result column lane & 15 (token), rows 4 (lane >> 4) .. + 3 (channels)
+#pragma unroll
+  for (int a = 0; a < TN; ++a)
+#pragma unroll
+    for (int b = 0; b < TM; ++b)
+      *reinterpret_cast<i32x4*>(&patch[wave][(16 * b + r16) * LD + 16 * a + 4 * g]) = acc[a][b];
+  sr.store(scales);
+  __syncthreads();
+  const int* patches[KW];
+#pragma unroll
+  for (int w = 0; w < KW; ++w) patches[w] = patch[w];
+  constexpr int LPR = BO / 8;
+  for (int e = tid; e < BM * LPR; e += 64 * KW) {
+    const int r = e / LPR, c = e % LPR * 8, pc = GLU ? c / 16 * 32 + c % 16 : c;
+    Lane8<GLU> ch;
+    ch.template read<16>(scales.sw + pc, scales.bias + pc);
+    if (p.vec) finish8<EL, GLU, KW, 16, true>(p, patches, r * LD + pc, scales.sx[r], ch, m0 + r, n0 + c, NO);
+    else finish8<EL, GLU, KW, 16, false>(p, patches, r * LD + pc, scales.sx[r], ch, m0 + r, n0 + c, NO);
   }
 }
 
@@ -466,6 +687,13 @@ ARB_API int arb_quantize_rows(const void* x, long ldx, const void* gamma, const 
   return (int)hipGetLastError();
 }
 
+template <int EL, bool GLU, int TM, int TN, int KW>
+static void launch_direct(const LinArgs& p, hipStream_t s) {
+  const int NO = GLU ? p.N / 2 : p.N, BO = GLU ? 8 * TN : 16 * TN;
+  const long tiles = (long)((p.M + 16 * TM - 1) / (16 * TM)) * ((NO + BO - 1) / BO);
+  linear_int8_direct_kernel<EL, GLU, TM, TN, KW><<<dim3((unsigned)tiles), 64 * KW, 0, s>>>(p);
+}
+
 template <int EL, bool GLU, int BM, int BN, int WM, int WN, int NS>
 static void launch_tiles(const LinArgs& p, hipStream_t s) {
   const int NO = GLU ? p.N / 2 : p.N, BO = GLU ? BN / 2 : BN;
@@ -473,24 +701,47 @@ static void launch_tiles(const LinArgs& p, hipStream_t s) {
   linear_int8_kernel<EL, GLU, BM, BN, WM, WN, NS><<<dim3((unsigned)tiles), 64 * WM * WN, 0, s>>>(p);
 }
 
+// Kernel by size (the sums are exact: every choice gives the same bits).  Measured, us, the product alone:
+//                              256x256  64x128 ring 2  64x128 ring 4  direct 16x32
+//   16384 x 8192 x 8192            918           1337           1544         10676
+//   65536 x 320 -> 960            49.9           57.5           97.7           287
+//   4096 x 1280 -> 1280           21.5           14.7           18.2          74.1
+//   1232 x 4096 -> 1024           47.1           20.2           14.0          55.3
+//   162 x 2048 -> 6144            26.7           11.9            8.5          27.8
+//   1 x 2048 -> 8192              24.9           11.8            8.6           6.2
+// 256 x 256 from one tile per CU on; below, 64 x 128 with two stages while two and more workgroups share a CU
+// and hide each other's latency, with four where a CU has one; up to 16 tokens the weight alone counts.
 template <int EL, bool GLU>
 static void launch_linear(const LinArgs& p, hipStream_t s) {
   auto tiles = [&](long bm, long bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-  if (tiles(256, 256) >= 256) launch_tiles<EL, GLU, 256, 256, 2, 4, 2>(p, s);
-  else if (tiles(128, 128) >= 256) launch_tiles<EL, GLU, 128, 128, 2, 2, 3>(p, s);
-  else launch_tiles<EL, GLU, 64, 128, 2, 2, 4>(p, s);
+  constexpr int WN = GLU ? 2 : 4;                                 // value and gate groups share a wave
+  if (p.M <= 16) launch_direct<EL, GLU, 1, 2, 8>(p, s);
+  else if (tiles(256, 256) >= 256) launch_tiles<EL, GLU, 256, 256, 2, 4, 2>(p, s);
+  else if (tiles(64, 128) >= 512) launch_tiles<EL, GLU, 64, 128, 2, WN, 2>(p, s);
+  else launch_tiles<EL, GLU, 64, 128, 2, WN, 4>(p, s);
 }
 
-ARB_API int arb_linear_int8(const void* x, long ldx, const void* sx, const void* w, long ldw, const void* sw,
-                            const void* b, const void* res, void* y, int M, int N, int K, int act, int el,
-                            hipStream_t stream) {
+// sx != null: x int8 rows (stride ldx bytes) with scales sx.  sx null: x 16-bit rows (stride ldx elements), which are
+// quantised (gamma / beta: LayerNorm first) into ws - M rows of K rounded up to 16 bytes, then M scales.
+ARB_API int arb_linear_int8(const void* x, long ldx, const void* sx, const void* gamma, const void* beta, float eps,
+                            void* ws, const void* w, long ldw, const void* sw, const void* b, const void* res,
+                            void* y, int M, int N, int K, int act, int el, hipStream_t stream) {
   const int kp = (K + 15) / 16 * 16;
-  if (M <= 0 || N <= 0 || K <= 0 || K > 133000 || ldx < kp || ldw < kp || ldx % 16 || ldw % 16 || act < 0 || act > 3 ||
-      (act == ACT_GEGLU && (N % 2 || res)))
+  if (M <= 0 || N <= 0 || K <= 0 || K > 133000 || ldw < kp || ldw % 16 || act < 0 || act > 3 ||
+      (act == ACT_GEGLU && (N % 2 || res)) || (sx == nullptr) != (ws != nullptr))
     return -1;
-  if (ldx >= (1L << 22) || ldw >= (1L << 22)) return -1;          // 31-bit byte offsets inside a tile
   LinArgs p{(const int8_t*)x, (const int8_t*)w, (const float*)sx, (const float*)sw, (const uint16_t*)b,
-            (const uint16_t*)res, (uint16_t*)y, ldx, ldw, M, N, K, act};
+            (const uint16_t*)res, (uint16_t*)y, ldx, ldw, M, N, K, act,
+            (act == ACT_GEGLU ? N / 2 : N) % 8 == 0 && (size_t)res % 16 == 0 && (size_t)y % 16 == 0};
+  if (sx == nullptr) {
+    float* scale = (float*)((int8_t*)ws + (size_t)M * kp);
+    const int rc = arb_quantize_rows(x, ldx, gamma, beta, eps, ws, kp, scale, M, K, el, stream);
+    if (rc != 0) return rc;
+    p.x = (const int8_t*)ws;
+    p.ldx = kp;
+    p.sx = scale;
+  }
+  if (p.ldx < kp || p.ldx % 16 || p.ldx >= (1L << 22) || ldw >= (1L << 22)) return -1;   // 31-bit offsets in a tile
   if (act == ACT_GEGLU) {
     if (el) launch_linear<1, true>(p, stream);
     else launch_linear<0, true>(p, stream);

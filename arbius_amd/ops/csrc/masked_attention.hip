@@ -552,12 +552,15 @@ ARB_API size_t arb_masked_attention_workspace(int B, long batch, int H, int Hkv,
   return s > 1 ? (size_t)s * B * H * Nq * (D + 2) * sizeof(float) : 0;
 }
 
-// strides: {q, k, v, o} x {batch, token, head} elements; ints: {B, H, Hkv, Nq, Nk, D, causal, q_start, n_docs,
-// docs_sb, prefix_sb, canonical batch}
-ARB_API int arb_masked_attention(const void* q, const void* k, const void* v, void* o, const long* strides,
-                                 const long* ints, const void* q_starts, const void* lengths, const void* docs,
-                                 const void* prefix, const void* slopes, void* ws, float scale, float softcap, int el,
+// dims: {q, k, v, o} x {batch, token, head} strides in elements, then {B, H, Hkv, Nq, Nk, D, causal, q_start,
+// n_docs, docs_sb, prefix_sb, canonical batch}
+ARB_API int arb_masked_attention(const void* q, const void* k, const void* v, void* o, const void* dims,
+                                 const void* q_starts, const void* lengths, const void* docs, const void* prefix,
+                                 const void* slopes, void* ws, float scale, float softcap, int el,
                                  hipStream_t stream) {
+  long strides[12], ints[12];
+  __builtin_memcpy(strides, dims, sizeof(strides));
+  __builtin_memcpy(ints, (const char*)dims + sizeof(strides), sizeof(ints));
   MaskedArgs a;
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v; a.o = (uint16_t*)o;
   a.q_sb = strides[0]; a.q_sn = strides[1]; a.q_sh = strides[2];
