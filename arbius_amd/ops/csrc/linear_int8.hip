@@ -73,10 +73,14 @@ __device__ __forceinline__ void dec8(uint4 v, float (&f)[8]) {
     f[2 * i + 1] = dec16<EL>(w[i] >> 16);
   }
 }
-// sum / maximum over the T threads (64: a wave, 256: the block) that share a row; fixed order
+// sum / maximum over the T threads that share a row (8 .. 64 lanes of a wave, or the block of 256); fixed order
 template <int T, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* red) {
-  v = MAX ? wave_max(v) : wave_sum(v);
+#pragma unroll
+  for (int o = T < 64 ? T / 2 : 32; o > 0; o >>= 1) {
+    const float u = __shfl_xor(v, o, 64);
+    v = MAX ? fmaxf(v, u) : v + u;
+  }
   if constexpr (T == 256) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -86,10 +90,9 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
   return v;
 }
 
-// One row per T threads (T = 64: four rows per workgroup), held in registers: V vectors of 8 elements per thread,
-// K <= 8 T V, K % 8 == 0, 16-byte aligned rows.  LN: LayerNorm in fp32 first (two exact passes over the
-// registers), the normalised row not rounded before it is quantised.  Bound by memory: 2 bytes read and 1
-// written per element in one pass.
+// One row per T threads, held in registers: V vectors of 8 elements per thread, K <= 8 T V, K % 8 == 0, 16-byte
+// aligned rows.  LN: LayerNorm in fp32 first (two exact passes over the registers), the normalised row not
+// rounded before it is quantised.  Bound by memory: 2 bytes read and 1 written per element in one pass.
 template <int EL, bool LN, int T, int V>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint16_t* __restrict__ x, long ldx,
                                                             const uint16_t* __restrict__ gamma,
@@ -99,7 +102,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint16_t* __re
   __shared__ float red[4];
   const int t = threadIdx.x % T;
   const long row = blockIdx.x * (256L / T) + threadIdx.x / T;
-  if (T == 64 && row >= rows) return;
+  if (T < 256 && row >= rows) return;
   const uint16_t* xr = x + row * ldx;
   const int NV = K >> 3;
   float f[V][8];
@@ -658,11 +661,17 @@ static void launch_quantize(const uint16_t* x, long ldx, const uint16_t* g, cons
 #define QROWS(T, V)                                                                                            \
   quantize_rows_kernel<EL, LN, T, V><<<dim3((unsigned)((rows + 256 / T - 1) / (256 / T))), 256, 0, stream>>>(   \
       x, ldx, g, b, eps, q, ldq, scale, rows, K)
+  // Lanes per row.  LN: by K alone (its sums' order must not depend on the rows of the batch), about 5 vectors a
+  // lane.  Without LN every choice gives the same bits: few rows are spread over whole workgroups.
+  const bool few = !LN && rows < 4096;
   if (!vec || nv > 2048)
     quantize_rows_any_kernel<EL, LN><<<dim3((unsigned)rows), 256, 0, stream>>>(x, ldx, g, b, eps, q, ldq, scale, K);
+  else if (nv <= 40 && !few) QROWS(8, 5);
+  else if (nv <= 80 && !few) QROWS(16, 5);
   else if (nv <= 64) QROWS(64, 1);
-  else if (nv <= 128) QROWS(64, 2);
-  else if (nv <= 256) QROWS(256, 1);
+  else if (nv <= 160 && !few) QROWS(32, 5);
+  else if (nv <= 256 && few) QROWS(256, 1);
+  else if (nv <= 320 && !few) QROWS(64, 5);
   else if (nv <= 512) QROWS(256, 2);
   else if (nv <= 1024) QROWS(256, 4);
   else QROWS(256, 8);
