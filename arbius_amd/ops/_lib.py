@@ -1206,8 +1206,8 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
         sb, sn, sh, sd = t.stride()
         if sd != 1 or (sb | sn | sh) % 8 or t.data_ptr() % 16:
             raise ValueError("masked_attention: last dim must be contiguous, strides/base 16B aligned")
-    # keys that share memory (a token stride below D) or lie 16 MiB apart are out of the tile loads' addressing
-    k, v = (t if D <= t.stride(1) < 1 << 23 else t.contiguous() for t in (k, v))
+    # keys that share memory (a token stride below D) or lie 8 MiB apart are out of the tile loads' addressing
+    k, v = (t if D <= t.stride(1) < 1 << 22 else t.contiguous() for t in (k, v))
     o = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
     if not o.numel():
         return o
