@@ -2,32 +2,29 @@
 // their own (masked_attention_f16.hip), the two compile side by side.
 #include "masked_attention.inc"
 
-int dispatch_masked_f16(const MaskedArgs& a, bool by_keys, hipStream_t s);
+int dispatch_masked_f16(const MaskedArgs& a, hipStream_t s);
 
 // How a call's keys are divided.  `batch`: the canonical batch under batch-invariant planning, so that a sequence's
 // parts do not depend on what shares its launch.
 struct KeyPlan {
-  bool by_keys;
-  int splits, parts;
+  int splits, wk;
 };
 static KeyPlan key_plan(long batch, int H, int Hkv, int Nq, int Nk, int D) {
-  const long rows = (long)(H / Hkv) * Nq;
-  // at most 32 rows and a cache worth it: waves over keys.  Wider heads do not fit two stages of 128 keys in LDS.
-  const bool by_keys = rows <= 32 && Nk >= 512 && D <= 128;
-  const long wgs = (by_keys ? 1 : (rows + 127) / 128) * Hkv * batch;
-  // split while the launch has fewer than two workgroups per CU (waves over keys: one) and a range keeps 256 keys
-  const long want = by_keys ? 256 : wgs < 128 ? 512 : 1;
-  long s = (want + wgs - 1) / wgs;
-  const long most = by_keys ? (Nk + 511) / 512 : (Nk + 255) / 256, cap = by_keys ? 16 : 64;
-  s = s < most ? s : most;
-  s = s < 1 ? 1 : s > cap ? cap : s;
-  return {by_keys, (int)s, (int)(by_keys ? 4 * s : s)};
+  const long rows = (long)(H / Hkv) * Nq, wgs = (rows + 127) / 128 * Hkv * batch;
+  // Key ranges (a second kernel joins them): up to two workgroups per CU, 128 keys each at least, and not where
+  // the partial sums written and read (8 D bytes a row and range) pass the keys and values read (4 D a key).
+  long s = (512 + wgs - 1) / wgs;
+  s = min(min(s, (Nk + 127L) / 128), min(256L, Nk / (2 * rows)));
+  s = max(s, 1L);
+  // 8 waves where a CU gets one workgroup and the chain of tiles is long
+  const int wk = wgs * s <= 256 && Nk >= 512 && rows > 32 && D <= 128 ? 2 : 1;
+  return {(int)s, wk};
 }
 
 // bytes of workspace (0: none)
 ARB_API size_t arb_masked_attention_workspace(int B, long batch, int H, int Hkv, int Nq, int Nk, int D) {
   const KeyPlan kp = key_plan(batch, H, Hkv, Nq, Nk, D);
-  return kp.parts > 1 ? (size_t)kp.parts * B * H * Nq * (D + 2) * sizeof(float) : 0;
+  return kp.splits > 1 ? (size_t)kp.splits * B * H * Nq * (D + 2) * sizeof(float) : 0;
 }
 
 // dims: {q, k, v, o} x {batch, token, head} strides in elements, then {B, H, Hkv, Nq, Nk, D, causal, q_start,
@@ -55,15 +52,15 @@ ARB_API int arb_masked_attention(const void* q, const void* k, const void* v, vo
   if (a.B <= 0 || a.Nq <= 0 || a.Nk <= 0 || a.H <= 0 || a.Hkv <= 0 || a.H % a.Hkv || a.D <= 0 || a.D % 8 ||
       a.D > 256 || ints[11] <= 0)
     return -1;
-  // a tile's rows (at most 128) are addressed by 31-bit byte offsets; its row range check needs rows apart
+  // a tile's keys (at most 128) are addressed by 31-bit byte offsets; its row range check needs rows apart
   if (a.k_sn < a.D || a.v_sn < a.D || a.k_sn >= (1L << 22) || a.v_sn >= (1L << 22)) return -1;
   const long rows = (long)a.B * a.H * a.Nq;
   const KeyPlan kp = key_plan(ints[11], a.H, a.Hkv, a.Nq, a.Nk, a.D);
   a.splits = kp.splits;
-  a.parts = kp.parts;
-  if ((long)(a.H / a.Hkv) * a.Nq > 0x7fffffffL - 256 || (rows + 127) * a.parts > 0x7fffffffL) return -1;
-  if (a.parts > 1 && ws == nullptr) return -1;
+  a.wk = kp.wk;
+  if ((long)(a.H / a.Hkv) * a.Nq > 0x7fffffffL - 256 || (rows + 127) * a.splits > 0x7fffffffL) return -1;
+  if (a.splits > 1 && ws == nullptr) return -1;
   a.po = (float*)ws;
-  a.pml = a.parts > 1 ? (float2*)((float*)ws + (size_t)a.parts * rows * a.D) : nullptr;
-  return el ? dispatch_masked_f16(a, kp.by_keys, stream) : dispatch_masked<0>(a, kp.by_keys, stream);
+  a.pml = a.splits > 1 ? (float2*)((float*)ws + (size_t)a.splits * rows * a.D) : nullptr;
+  return el ? dispatch_masked_f16(a, stream) : dispatch_masked<0>(a, stream);
 }
