@@ -96,6 +96,7 @@ _SIGS = {
                                   c_int, c_int, c_void_p]),
     "arb_linear_int8": (c_int, [c_void_p, c_long] + [c_void_p] * 3 + [c_float] + [c_void_p] * 2 + [c_long]
                         + [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
+    "arb_linear_int8_few": (c_int, [c_void_p, c_long, c_int, c_int]),
     "arb_masked_attention": (c_int, [c_void_p] * 4 + [ctypes.c_char_p] + [c_void_p] * 6 + [c_float, c_float, c_int,
                                                                                           c_void_p]),
     "arb_masked_attention_workspace": (c_size_t, [c_int, c_long] + [c_int] * 5),
@@ -138,7 +139,7 @@ _AUDIT = None
 _HOST_SYMBOLS = ("arb_conv2d_plan", "arb_conv_family", "arb_conv2d_workspace", "arb_group_norm_workspace",
                  "arb_group_norm_slice_ok",
                  "arb_rvm_args_sizes", "arb_attention512_workspace", "arb_h264_intra_workspace",
-                 "arb_h264_intra_host", "arb_masked_attention_workspace")
+                 "arb_h264_intra_host", "arb_masked_attention_workspace", "arb_linear_int8_few")
 
 
 def auditing() -> bool:
@@ -1184,11 +1185,12 @@ def _linear_int8(x, sx, norm, w, sw, b, residual, act, shape, dtype):
         audit_note("linear_int8", M=M, N=N, K=K)
     if not M or not N:
         return y
-    ws = None
-    if sx is None:                 # int8 rows of a multiple of 16 bytes, then the scales
+    ws, px = None, x2.data_ptr()
+    # int8 rows of a multiple of 16 bytes, then the scales - but for few tokens, quantised inside the kernel
+    if sx is None and (M > 4 or norm is not None or not _fn("arb_linear_int8_few")(px, ldx, M, K)):
         ws = torch.empty(M * ((K + 15) // 16 * 16 + 4), dtype=torch.uint8, device=w.device)
     gamma, beta, eps = norm if norm is not None else (None, None, 0.0)
-    _check(_launch(w, _fn("arb_linear_int8"), x2.data_ptr(), ldx, _ptr(sx), _ptr(gamma), _ptr(beta), eps, _ptr(ws),
+    _check(_launch(w, _fn("arb_linear_int8"), px, ldx, _ptr(sx), _ptr(gamma), _ptr(beta), eps, _ptr(ws),
                    w.data_ptr(), w.stride(0), sw.data_ptr(), _ptr(b), _ptr(residual), y.data_ptr(), M, N, K,
                    _INT8_ACT[act], el), "linear_int8")
     return y

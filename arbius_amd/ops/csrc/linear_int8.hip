@@ -260,7 +260,7 @@ struct ScaleRegs {
 #pragma unroll
     for (int i = 0; i < NX; ++i) {
       const int m = m0 + (int)threadIdx.x + NT * i;
-      sx[i] = p.sx[min(m, p.M - 1)];
+      sx[i] = p.sx ? p.sx[min(m, p.M - 1)] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NWR; ++i) {
@@ -269,10 +269,10 @@ struct ScaleRegs {
       bias[i] = p.b ? p.b[n] : 0;
     }
   }
-  __device__ __forceinline__ void store(TileScales<BM, BN>& t) const {
+  __device__ __forceinline__ void store(TileScales<BM, BN>& t, bool tokens = true) const {
 #pragma unroll
     for (int i = 0; i < NX; ++i)
-      if ((int)threadIdx.x + NT * i < BM) t.sx[threadIdx.x + NT * i] = sx[i];
+      if (tokens && (int)threadIdx.x + NT * i < BM) t.sx[threadIdx.x + NT * i] = sx[i];
 #pragma unroll
     for (int i = 0; i < NWR; ++i)
       if ((int)threadIdx.x + NT * i < BN) {
@@ -556,43 +556,52 @@ __device__ __forceinline__ uint4 load_i8(const int8_t* base, unsigned off, int k
   return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, k0, 0));
 }
 
-// Few tokens: 16 TM tokens x 16 TN weight rows per workgroup, and its KW waves split K.  No LDS and no barrier in the
-// loop: each wave keeps two K tiles of 128 bytes of both operands in flight in its own registers, a lane's
-// 16 bytes being its 16x16x64 MFMA fragment as it lies in memory.  The integer partial sums of the waves meet
-// in LDS.  Bound by the read of the weight: 1 x 2048 -> 8192 in 6.2 us, 2.7 TB/s.
-template <int EL, bool GLU, int TM, int TN, int KW>
-__global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs p) {
-  constexpr int BM = 16 * TM, BN = 16 * TN, BO = GLU ? BN / 2 : BN, LD = BN + 4;
+// Few tokens (at most 16): 16 TN weight rows per workgroup, and its KW waves split K.  No LDS-DMA and no barrier in the
+// loop: each wave keeps two K tiles of 128 bytes in flight in its own registers, a lane's 16 bytes being its
+// 16x16x64 MFMA fragment as it lies in memory.  The integer partial sums of the waves meet in LDS.
+// MR > 0 (at most MR tokens, K <= 8192): x comes in 16 bits and every workgroup quantises it for itself, into LDS,
+// while its weights are on their way - a few KB from the L2 instead of a launch.  The quantisation is exact, so
+// this gives the bits of quantize_rows.
+// Bound by the read of the weight: 1 x 2048 -> 8192 in 6.2 us, 2.7 TB/s (8.3 with the quantisation launched apart).
+template <int EL, bool GLU, int TN, int KW, int MR>
+__global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs p, const uint16_t* __restrict__ x16,
+                                                                        long ldx16) {
+  constexpr int BM = 16, BN = 16 * TN, BO = GLU ? BN / 2 : BN, LD = BN + 4, NT = 64 * KW;
+  constexpr int KMAX = 8192, QLD = KMAX + 16;                     // (16 bytes apart: rows start on other banks)
   static_assert(!GLU || TN % 2 == 0, "value and gate groups");
+  static_assert(MR == 0 || KMAX / 8 <= 2 * NT, "two vectors a thread");
   __shared__ __attribute__((aligned(16))) int patch[KW][BM * LD];
+  __shared__ __attribute__((aligned(16))) int8_t sq[MR ? MR * QLD : 16];
+  __shared__ float sred[MR ? MR : 1][KW];
   __shared__ TileScales<BM, BN> scales;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int NO = GLU ? p.N / 2 : p.N;
-  int m0, n0;
-  tile_of((p.M + BM - 1) / BM, (NO + BO - 1) / BO, m0, n0);
-  m0 *= BM;
-  n0 *= BO;
-  // rows past the last one repeat it: their results are not stored.  GLU: 16-row groups alternate values and gates
-  unsigned xo[TM], wo[TN];
+  const int n0 = xcd_remap(blockIdx.x, (NO + BO - 1) / BO) * BO;
+  const int kp = (p.K + 15) & ~15, nk = (kp + 127) / 128;
+
+  uint4 xv[MR ? MR : 1][2];
+  if constexpr (MR > 0) {                                         // before the weights: loads return in order
 #pragma unroll
-  for (int b = 0; b < TM; ++b) xo[b] = (unsigned)(min(16 * b + r16, p.M - 1 - m0) * (int)p.ldx + 16 * g);
+    for (int r = 0; r < MR; ++r)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int v = tid + NT * j;
+        xv[r][j] = 8 * v < p.K ? ld16(x16 + min(r, p.M - 1) * ldx16 + 8 * v) : make_uint4(0, 0, 0, 0);
+      }
+  }
+  // rows past the last one repeat it: their results are not stored.  GLU: 16-row groups alternate values and gates
+  const unsigned xo = MR ? 0u : (unsigned)(min(r16, p.M - 1) * (int)p.ldx + 16 * g);
+  unsigned wo[TN];
 #pragma unroll
   for (int a = 0; a < TN; ++a) {
     const int r = GLU ? 16 * (a >> 1) + r16 : 16 * a + r16;
     wo[a] = (unsigned)(min(r, NO - 1 - n0) * (int)p.ldw + 16 * g);
   }
-  ScaleRegs<EL, BM, BN, 64 * KW> sr;
-  sr.load(p, m0, [&](int r) {
-    const int n = GLU ? n0 + (r >> 5) * 16 + (r & 15) : n0 + r;
-    return n >= NO ? -1 : GLU && ((r >> 4) & 1) ? NO + n : n;
-  });
-  const int kp = (p.K + 15) & ~15, nk = (kp + 127) / 128;
-  const int8_t* xb = p.x + (long)m0 * p.ldx;
   const int8_t* wb = p.w + (long)n0 * p.ldw;
   const int8_t* gb = GLU ? wb + (long)NO * p.ldw : wb;
 
-  uint4 xf[2][2][TM], wf[2][2][TN];
+  uint4 xf[2][2], wf[2][2][TN];
   auto load = [&](auto buf, int kt) __attribute__((always_inline)) {
     constexpr int B = decltype(buf)::value;
 #pragma unroll
@@ -600,56 +609,94 @@ __global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs 
       const int k0 = 128 * kt + 64 * s;
       const unsigned past = k0 + 16 * g < kp ? 0u : kZeros;       // chunks behind the row
 #pragma unroll
-      for (int a = 0; a < TN; ++a)
-        wf[B][s][a] = load_i8(GLU && (a & 1) ? gb : wb, wo[a] | past, k0);
-#pragma unroll
-      for (int b = 0; b < TM; ++b) xf[B][s][b] = load_i8(xb, xo[b] | past, k0);
+      for (int a = 0; a < TN; ++a) wf[B][s][a] = load_i8(GLU && (a & 1) ? gb : wb, wo[a] | past, k0);
+      if constexpr (MR == 0) xf[B][s] = load_i8(p.x, xo | past, k0);
     }
-  };
-  i32x4 acc[TN][TM];
-#pragma unroll
-  for (int a = 0; a < TN; ++a)
-#pragma unroll
-    for (int b = 0; b < TM; ++b) acc[a][b] = (i32x4){};
-  auto mma = [&](auto buf) __attribute__((always_inline)) {
-    constexpr int B = decltype(buf)::value;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int a = 0; a < TN; ++a)
-#pragma unroll
-        for (int b = 0; b < TM; ++b)
-          acc[a][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[B][s][a]),
-                                                            __builtin_bit_cast(i32x4, xf[B][s][b]), acc[a][b], 0, 0, 0);
   };
   if (wave < nk) load(Stage<0>(), wave);
   if (wave + KW < nk) load(Stage<1>(), wave + KW);
+  ScaleRegs<EL, BM, BN, NT> sr;
+  sr.load(p, 0, [&](int r) {
+    const int n = GLU ? n0 + (r >> 5) * 16 + (r & 15) : n0 + r;
+    return n >= NO ? -1 : GLU && ((r >> 4) & 1) ? NO + n : n;
+  });
+  if constexpr (MR > 0) {
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+      float a = 0.f;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float f[8];
+        dec8<EL>(xv[r][j], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          bad |= f[e] != f[e];
+          a = fmaxf(a, fabsf(f[e]));
+        }
+      }
+      a = wave_max(bad ? INFINITY : a);
+      if (lane == 0) sred[r][wave] = a;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+      float a = sred[r][0];
+#pragma unroll
+      for (int w = 1; w < KW; ++w) a = fmaxf(a, sred[r][w]);
+      float s, inv, up;
+      quant_scale(a, s, inv, up);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int v = tid + NT * j;
+        if (8 * v < 128 * nk) {                                   // zeros to the end of the last K tile
+          float f[8];
+          dec8<EL>(xv[r][j], f);
+          *reinterpret_cast<uint2*>(sq + r * QLD + 8 * v) = inv != 0.f ? quant8(f, inv, up) : make_uint2(0u, 0u);
+        }
+      }
+      if (tid == 0) scales.sx[r] = s;
+    }
+    __syncthreads();
+  }
+  i32x4 acc[TN];
+#pragma unroll
+  for (int a = 0; a < TN; ++a) acc[a] = (i32x4){};
+  auto mma = [&](auto buf, int kt) __attribute__((always_inline)) {
+    constexpr int B = decltype(buf)::value;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if constexpr (MR > 0) xf[B][s] = ld16(sq + min(r16, MR - 1) * QLD + 128 * kt + 64 * s + 16 * g);
+#pragma unroll
+      for (int a = 0; a < TN; ++a)
+        acc[a] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[B][s][a]),
+                                                       __builtin_bit_cast(i32x4, xf[B][s]), acc[a], 0, 0, 0);
+    }
+  };
   for (int kt = wave; kt < nk; kt += 2 * KW) {
-    mma(Stage<0>());
+    mma(Stage<0>(), kt);
     if (kt + 2 * KW < nk) load(Stage<0>(), kt + 2 * KW);
     if (kt + KW < nk) {
-      mma(Stage<1>());
+      mma(Stage<1>(), kt + KW);
       if (kt + 3 * KW < nk) load(Stage<1>(), kt + 3 * KW);
     }
   }
   // result column lane & 15 (token), rows 4 (lane >> 4) .. + 3 (channels)
 #pragma unroll
-  for (int a = 0; a < TN; ++a)
-#pragma unroll
-    for (int b = 0; b < TM; ++b)
-      *reinterpret_cast<i32x4*>(&patch[wave][(16 * b + r16) * LD + 16 * a + 4 * g]) = acc[a][b];
-  sr.store(scales);
+  for (int a = 0; a < TN; ++a) *reinterpret_cast<i32x4*>(&patch[wave][r16 * LD + 16 * a + 4 * g]) = acc[a];
+  sr.store(scales, MR == 0);
   __syncthreads();
   const int* patches[KW];
 #pragma unroll
   for (int w = 0; w < KW; ++w) patches[w] = patch[w];
   constexpr int LPR = BO / 8;
-  for (int e = tid; e < BM * LPR; e += 64 * KW) {
+  for (int e = tid; e < BM * LPR; e += NT) {
     const int r = e / LPR, c = e % LPR * 8, pc = GLU ? c / 16 * 32 + c % 16 : c;
+    if (r >= p.M) break;
     Lane8<GLU> ch;
     ch.template read<16>(scales.sw + pc, scales.bias + pc);
-    if (p.vec) finish8<EL, GLU, KW, 16, true>(p, patches, r * LD + pc, scales.sx[r], ch, m0 + r, n0 + c, NO);
-    else finish8<EL, GLU, KW, 16, false>(p, patches, r * LD + pc, scales.sx[r], ch, m0 + r, n0 + c, NO);
+    if (p.vec) finish8<EL, GLU, KW, 16, true>(p, patches, r * LD + pc, scales.sx[r], ch, r, n0 + c, NO);
+    else finish8<EL, GLU, KW, 16, false>(p, patches, r * LD + pc, scales.sx[r], ch, r, n0 + c, NO);
   }
 }
 
@@ -696,11 +743,10 @@ ARB_API int arb_quantize_rows(const void* x, long ldx, const void* gamma, const 
   return (int)hipGetLastError();
 }
 
-template <int EL, bool GLU, int TM, int TN, int KW>
-static void launch_direct(const LinArgs& p, hipStream_t s) {
-  const int NO = GLU ? p.N / 2 : p.N, BO = GLU ? 8 * TN : 16 * TN;
-  const long tiles = (long)((p.M + 16 * TM - 1) / (16 * TM)) * ((NO + BO - 1) / BO);
-  linear_int8_direct_kernel<EL, GLU, TM, TN, KW><<<dim3((unsigned)tiles), 64 * KW, 0, s>>>(p);
+template <int EL, bool GLU, int MR>
+static void launch_direct(const LinArgs& p, hipStream_t s, const uint16_t* x16 = nullptr, long ldx16 = 0) {
+  const int NO = GLU ? p.N / 2 : p.N, BO = GLU ? 16 : 32;
+  linear_int8_direct_kernel<EL, GLU, 2, 8, MR><<<dim3((unsigned)((NO + BO - 1) / BO)), 512, 0, s>>>(p, x16, ldx16);
 }
 
 template <int EL, bool GLU, int BM, int BN, int WM, int WN, int NS>
@@ -724,25 +770,47 @@ template <int EL, bool GLU>
 static void launch_linear(const LinArgs& p, hipStream_t s) {
   auto tiles = [&](long bm, long bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   constexpr int WN = GLU ? 2 : 4;                                 // value and gate groups share a wave
-  if (p.M <= 16) launch_direct<EL, GLU, 1, 2, 8>(p, s);
+  if (p.M <= 16) launch_direct<EL, GLU, 0>(p, s);
   else if (tiles(256, 256) >= 256) launch_tiles<EL, GLU, 256, 256, 2, 4, 2>(p, s);
   else if (tiles(64, 128) >= 512) launch_tiles<EL, GLU, 64, 128, 2, WN, 2>(p, s);
   else launch_tiles<EL, GLU, 64, 128, 2, WN, 4>(p, s);
 }
 
+// Whether a product of 16-bit rows without LayerNorm quantises them itself: up to 4 tokens.  (Behind a LayerNorm the
+// sums would run in another order than for longer batches.)
+ARB_API int arb_linear_int8_few(const void* x, long ldx, int M, int K) {
+  return M <= 4 && K <= 8192 && K % 8 == 0 && ldx % 8 == 0 && (size_t)x % 16 == 0;
+}
+
 // sx != null: x int8 rows (stride ldx bytes) with scales sx.  sx null: x 16-bit rows (stride ldx elements), which are
-// quantised (gamma / beta: LayerNorm first) into ws - M rows of K rounded up to 16 bytes, then M scales.
+// quantised (gamma / beta: LayerNorm first) into ws - M rows of K rounded up to 16 bytes, then M scales (unused, may be
+// null, where arb_linear_int8_few says 1).
 ARB_API int arb_linear_int8(const void* x, long ldx, const void* sx, const void* gamma, const void* beta, float eps,
                             void* ws, const void* w, long ldw, const void* sw, const void* b, const void* res,
                             void* y, int M, int N, int K, int act, int el, hipStream_t stream) {
   const int kp = (K + 15) / 16 * 16;
   if (M <= 0 || N <= 0 || K <= 0 || K > 133000 || ldw < kp || ldw % 16 || act < 0 || act > 3 ||
-      (act == ACT_GEGLU && (N % 2 || res)) || (sx == nullptr) != (ws != nullptr))
+      (act == ACT_GEGLU && (N % 2 || res)))
     return -1;
   LinArgs p{(const int8_t*)x, (const int8_t*)w, (const float*)sx, (const float*)sw, (const uint16_t*)b,
             (const uint16_t*)res, (uint16_t*)y, ldx, ldw, M, N, K, act,
             (act == ACT_GEGLU ? N / 2 : N) % 8 == 0 && (size_t)res % 16 == 0 && (size_t)y % 16 == 0};
+  if (ldw >= (1L << 22)) return -1;                               // 31-bit offsets in a tile
+  if (sx == nullptr && !gamma && arb_linear_int8_few(x, ldx, M, K)) {
+    const uint16_t* x16 = (const uint16_t*)x;
+#define FEW(EL, GLU)                                       \
+  if (M == 1) launch_direct<EL, GLU, 1>(p, stream, x16, ldx); \
+  else launch_direct<EL, GLU, 4>(p, stream, x16, ldx)
+    if (act == ACT_GEGLU) {
+      if (el) { FEW(1, true); } else { FEW(0, true); }
+    } else {
+      if (el) { FEW(1, false); } else { FEW(0, false); }
+    }
+#undef FEW
+    return (int)hipGetLastError();
+  }
   if (sx == nullptr) {
+    if (ws == nullptr) return -1;
     float* scale = (float*)((int8_t*)ws + (size_t)M * kp);
     const int rc = arb_quantize_rows(x, ldx, gamma, beta, eps, ws, kp, scale, M, K, el, stream);
     if (rc != 0) return rc;
@@ -750,7 +818,7 @@ ARB_API int arb_linear_int8(const void* x, long ldx, const void* sx, const void*
     p.ldx = kp;
     p.sx = scale;
   }
-  if (p.ldx < kp || p.ldx % 16 || p.ldx >= (1L << 22) || ldw >= (1L << 22)) return -1;   // 31-bit offsets in a tile
+  if (p.ldx < kp || p.ldx % 16 || p.ldx >= (1L << 22)) return -1;
   if (act == ACT_GEGLU) {
     if (el) launch_linear<1, true>(p, stream);
     else launch_linear<0, true>(p, stream);

@@ -341,3 +341,67 @@ def test_more_rows_than_a_grid_dimension(cuda):
     w = rows(40, 48, 2, cuda)
     y = ops.linear_int8(x, w)
     assert torch.equal(y[:64].repeat(-(-m // 64), 1)[:m], y)
+
+
+# ------------------------------------------------------------------ few tokens
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", [None, "geglu"])
+@pytest.mark.parametrize("k,n", [(8, 2), (72, 34), (640, 520), (2048, 96), (8184, 66), (8192, 40), (8200, 40), (77, 30)])
+def test_few_tokens(device, dtype, act, k, n):
+    """1 to 17 tokens around every switch of kernels: rows quantised inside the product or apart give the same bits,
+    also zero rows, rows with NaN or infinity, and rows cut out of wider ones."""
+    dt = DTYPES[dtype]
+    wide = randn(17, k + 24, seed=k, dtype=dt, device=device)
+    wide[2], wide[3, 9] = 0, float("nan")
+    if k > 8:
+        wide[1, -25], wide[5, 8] = float("inf"), -float("inf")
+    w, b = rows(n, k, n, device, dt), randn(n, seed=1, dtype=dt, device=device)
+    for m in (1, 2, 3, 4, 5, 17):
+        for x in (wide[:m, 8:8 + k], wide[:m, 3:3 + k], wide[17 - m:, 8:8 + k].clone(), wide[2:3, 8:8 + k]):
+            qx = ops.quantize_rows(x)
+            y = ops.linear_int8(x, w, b, act=act)
+            assert torch.equal(y.nan_to_num(7.0), ops.linear_int8(qx, w, b, act=act).nan_to_num(7.0))
+            fine = qx.scale.isfinite().cpu()
+            assert torch.equal(y.cpu().isnan().any(dim=1), ~fine)
+            check(y.cpu()[fine], *linear64(qx.q.cpu()[fine], qx.scale.cpu()[fine], w.q.cpu(), w.scale.cpu(), b.cpu(),
+                                           None, act))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("k", [320, 2048, 1001])
+def test_layernorm_batch_invariance(device, k):
+    x = randn(300, k, seed=1, dtype=torch.bfloat16, device=device)
+    gamma, beta = (1 + 0.1 * randn(k, seed=2)).to(x), (0.1 * randn(k, seed=3)).to(x)
+    w = rows(72, k, 4, device)
+    y, q = ops.ln_linear_int8(x, gamma, beta, 1e-5, w), ops.ln_quantize_rows(x, gamma, beta, 1e-5)
+    for a, e in ((0, 1), (7, 8), (20, 24), (3, 70), (100, 300)):
+        assert torch.equal(ops.ln_linear_int8(x[a:e], gamma, beta, 1e-5, w), y[a:e])
+        part = ops.ln_quantize_rows(x[a:e], gamma, beta, 1e-5)
+        assert torch.equal(part.q, q.q[a:e]) and torch.equal(part.scale, q.scale[a:e])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_operands_of_any_alignment(device):
+    """Bias and residual cut out of others at odd elements, results whose width is no multiple of a vector."""
+    for m, k, n in ((3, 64, 70), (70, 200, 136), (300, 128, 520)):
+        x, w = randn(m, k, seed=1, dtype=torch.bfloat16, device=device), rows(n, k, 2, device)
+        b = randn(n + 1, seed=3, dtype=torch.bfloat16, device=device)[1:]
+        store = randn(m * n + 3, seed=4, dtype=torch.bfloat16, device=device)
+        for r in (store[3:].view(m, n), store[1:1 + m * n].view(n, m).t(), store[:n].expand(m, n)):
+            y = ops.linear_int8(x, w, b, residual=r)
+            assert torch.equal(y, ops.linear_int8(x, w, b.clone(), residual=r.contiguous()))
+
+
+@pytest.mark.gpu
+def test_few_tokens_in_a_graph(cuda):
+    x, w = randn(2, 640, seed=1, dtype=torch.float16, device=cuda), rows(384, 640, 2, cuda, torch.float16)
+    ops.linear_int8(x, w)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.linear_int8(x, w)
+    for step in range(4):
+        x.copy_(randn(2, 640, seed=5 + step, dtype=torch.float16))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.linear_int8(ops.quantize_rows(x), w))
