@@ -305,7 +305,7 @@ def ln_linear_geglu(x, gamma, beta, eps, w, b=None):
 
 
 # --------------------------------------------------------------------------- 8-bit linears
-INT8_MAX_K = 133000          # 127^2 K stays below 2^31: the integer sums never wrap
+INT8_MAX_K = 131071          # 128^2 K stays below 2^31: the integer sums never wrap
 
 
 class Int8Rows:
@@ -343,8 +343,8 @@ class Int8Rows:
 
 
 def _quantize(x, norm, op):
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= INT8_MAX_K:
-        raise ValueError(f"{op}: x {tuple(x.shape)} (a last dim of 1 .. {INT8_MAX_K} expected)")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= INT8_MAX_K or x.numel() // x.shape[-1] >= 2 ** 31:
+        raise ValueError(f"{op}: x {tuple(x.shape)} (a last dim of 1 .. {INT8_MAX_K}, below 2^31 rows expected)")
     if not x.is_floating_point():
         raise TypeError(f"{op}: got {x.dtype}")
     if torch.is_grad_enabled() and x.requires_grad:
@@ -408,7 +408,7 @@ def _linear_int8_args(x, xshape, w, b, residual, act, op):
         raise TypeError(f"{op}: w must be the Int8Rows of a weight [N, K]")
     N, K = w.shape
     device, shape = w.q.device, tuple(xshape[:-1])
-    if xshape[-1] != K or x.device != device:
+    if xshape[-1] != K or x.device != device or max(math.prod(shape), N) >= 2 ** 31:
         raise ValueError(f"{op}: x {tuple(xshape)} on {x.device}, w {w.shape} on {device}")
     if act is not None and act not in _lib._INT8_ACT:
         raise ValueError(f"{op}: act {act!r}")
@@ -812,7 +812,8 @@ def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=No
     * ``documents`` int32 [n + 1] (or [B, n + 1]): offsets of n documents packed end to end; a query sees
       only keys of the document that holds its position (outside of all: nothing)
     * ``prefix`` int32 [B], or with ``documents`` [n] (or [B, n]): needs ``causal``
-    * ``softcap``: cap of the scores;  ``slopes`` fp32 [H]: linear bias by distance
+    * ``softcap``: cap of the scores, 2^-10 to 2^10 (they are off by 2^-21 of it)
+    * ``slopes`` fp32 [H]: linear bias by distance
 
     GPU: bf16 / fp16, D % 8 == 0, D <= 256 (csrc/masked_attention.hip).  Inference only."""
     qs, ks, dtype, device = q.shape, k.shape, q.dtype, q.device
@@ -826,10 +827,10 @@ def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=No
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("masked_attention: inference only (no gradients)")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if not abs(scale) <= 2.0 ** 20:
         raise ValueError(f"masked_attention: scale {scale}")
-    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
-        raise ValueError(f"masked_attention: softcap {softcap} (a positive number expected)")
+    if softcap is not None and not 2.0 ** -10 <= softcap <= 2.0 ** 10:
+        raise ValueError(f"masked_attention: softcap {softcap} (2^-10 to 2^10 expected)")
     if isinstance(q_start, torch.Tensor):
         _index_arg("q_start", q_start, q, [(B,)])
     else:
@@ -851,8 +852,8 @@ def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=No
     if slopes is not None and (not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32
                                or slopes.device != device or slopes.shape != (H,) or not slopes.is_contiguous()):
         raise ValueError(f"masked_attention: slopes must be contiguous fp32 [{H}] on {device}")
-    if Nq >= 2 ** 31 or ks[1] >= 2 ** 31:
-        raise ValueError("masked_attention: more than 2^31 - 1 queries or keys")
+    if max(B, H, Nq, ks[1], n) > 2 ** 31 - 1024:
+        raise ValueError(f"masked_attention: q {tuple(qs)} k / v {tuple(ks)} pass 2^31")
     args = (q, k, v, scale, bool(causal), q_start, lengths, prefix, documents, softcap, slopes)
     return _lib.masked_attention(*args, _canon_batch(B)) if _hip(q) else ref.masked_attention(*args)
 

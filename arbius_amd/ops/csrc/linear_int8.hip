@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs 
 }
 
 template <int EL, bool LN>
-static void launch_quantize(const uint16_t* x, long ldx, const uint16_t* g, const uint16_t* b, float eps, int8_t* q,
+static int launch_quantize(const uint16_t* x, long ldx, const uint16_t* g, const uint16_t* b, float eps, int8_t* q,
                             int ldq, float* scale, long rows, int K, hipStream_t stream) {
   const bool vec = K % 8 == 0 && ldx % 8 == 0 && (size_t)x % 16 == 0 && (size_t)g % 16 == 0 && (size_t)b % 16 == 0;
   const int nv = (ldq + 7) / 8;                                   // vectors a row's threads write
@@ -710,8 +710,10 @@ static void launch_quantize(const uint16_t* x, long ldx, const uint16_t* g, cons
       x, ldx, g, b, eps, q, ldq, scale, rows, K)
   // Lanes per row.  LN: by K alone (its sums' order must not depend on the rows of the batch), about 5 vectors a
   // lane.  Without LN every choice gives the same bits: few rows are spread over whole workgroups.
-  const bool few = !LN && rows < 4096;
-  if (!vec || nv > 2048)
+  const bool few = !LN && rows < 4096, any = !vec || nv > 2048;
+  // a launch has fewer than 2^32 threads
+  if (rows * (any || nv > 320 ? 256 : nv > 160 ? 64 : nv > 80 ? 32 : nv > 40 ? 16 : 8) >= (1L << 32) - 256) return -1;
+  if (any)
     quantize_rows_any_kernel<EL, LN><<<dim3((unsigned)rows), 256, 0, stream>>>(x, ldx, g, b, eps, q, ldq, scale, K);
   else if (nv <= 40 && !few) QROWS(8, 5);
   else if (nv <= 80 && !few) QROWS(16, 5);
@@ -723,6 +725,7 @@ static void launch_quantize(const uint16_t* x, long ldx, const uint16_t* g, cons
   else if (nv <= 1024) QROWS(256, 4);
   else QROWS(256, 8);
 #undef QROWS
+  return (int)hipGetLastError();
 }
 
 // x [rows, K] 16-bit (row stride ldx elements) -> q [rows, ldq] int8, scale [rows]; gamma / beta: LayerNorm first
@@ -733,27 +736,30 @@ ARB_API int arb_quantize_rows(const void* x, long ldx, const void* gamma, const 
     return -1;
   const uint16_t *xp = (const uint16_t*)x, *g = (const uint16_t*)gamma, *b = (const uint16_t*)beta;
 #define QUANT(EL, LN) \
-  launch_quantize<EL, LN>(xp, ldx, g, b, eps, (int8_t*)q, ldq, (float*)scale, rows, K, stream)
+  return launch_quantize<EL, LN>(xp, ldx, g, b, eps, (int8_t*)q, ldq, (float*)scale, rows, K, stream)
   if (gamma) {
     if (el) QUANT(1, true); else QUANT(0, true);
   } else {
     if (el) QUANT(1, false); else QUANT(0, false);
   }
 #undef QUANT
-  return (int)hipGetLastError();
 }
 
 template <int EL, bool GLU, int MR>
-static void launch_direct(const LinArgs& p, hipStream_t s, const uint16_t* x16 = nullptr, long ldx16 = 0) {
+static int launch_direct(const LinArgs& p, hipStream_t s, const uint16_t* x16 = nullptr, long ldx16 = 0) {
   const int NO = GLU ? p.N / 2 : p.N, BO = GLU ? 16 : 32;
+  if (NO >= 1 << 26) return -1;                                   // a launch has fewer than 2^32 threads
   linear_int8_direct_kernel<EL, GLU, 2, 8, MR><<<dim3((unsigned)((NO + BO - 1) / BO)), 512, 0, s>>>(p, x16, ldx16);
+  return (int)hipGetLastError();
 }
 
 template <int EL, bool GLU, int BM, int BN, int WM, int WN, int NS>
-static void launch_tiles(const LinArgs& p, hipStream_t s) {
+static int launch_tiles(const LinArgs& p, hipStream_t s) {
   const int NO = GLU ? p.N / 2 : p.N, BO = GLU ? BN / 2 : BN;
-  const long tiles = (long)((p.M + BM - 1) / BM) * ((NO + BO - 1) / BO);
+  const long tiles = ((p.M + BM - 1L) / BM) * ((NO + BO - 1L) / BO);
+  if (tiles * 64 * WM * WN >= (1L << 32)) return -1;              // a launch has fewer threads
   linear_int8_kernel<EL, GLU, BM, BN, WM, WN, NS><<<dim3((unsigned)tiles), 64 * WM * WN, 0, s>>>(p);
+  return (int)hipGetLastError();
 }
 
 // Kernel by size (the sums are exact: every choice gives the same bits).  Measured, us, the product alone:
@@ -767,13 +773,13 @@ static void launch_tiles(const LinArgs& p, hipStream_t s) {
 // 256 x 256 from one tile per CU on; below, 64 x 128 with two stages while two and more workgroups share a CU
 // and hide each other's latency, with four where a CU has one; up to 16 tokens the weight alone counts.
 template <int EL, bool GLU>
-static void launch_linear(const LinArgs& p, hipStream_t s) {
+static int launch_linear(const LinArgs& p, hipStream_t s) {
   auto tiles = [&](long bm, long bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   constexpr int WN = GLU ? 2 : 4;                                 // value and gate groups share a wave
-  if (p.M <= 16) launch_direct<EL, GLU, 0>(p, s);
-  else if (tiles(256, 256) >= 256) launch_tiles<EL, GLU, 256, 256, 2, 4, 2>(p, s);
-  else if (tiles(64, 128) >= 512) launch_tiles<EL, GLU, 64, 128, 2, WN, 2>(p, s);
-  else launch_tiles<EL, GLU, 64, 128, 2, WN, 4>(p, s);
+  if (p.M <= 16) return launch_direct<EL, GLU, 0>(p, s);
+  if (tiles(256, 256) >= 256) return launch_tiles<EL, GLU, 256, 256, 2, 4, 2>(p, s);
+  if (tiles(64, 128) >= 512) return launch_tiles<EL, GLU, 64, 128, 2, WN, 2>(p, s);
+  return launch_tiles<EL, GLU, 64, 128, 2, WN, 4>(p, s);
 }
 
 // Whether a product of 16-bit rows without LayerNorm quantises them itself: up to 4 tokens.  (Behind a LayerNorm the
@@ -789,7 +795,7 @@ ARB_API int arb_linear_int8(const void* x, long ldx, const void* sx, const void*
                             void* ws, const void* w, long ldw, const void* sw, const void* b, const void* res,
                             void* y, int M, int N, int K, int act, int el, hipStream_t stream) {
   const int kp = (K + 15) / 16 * 16;
-  if (M <= 0 || N <= 0 || K <= 0 || K > 133000 || ldw < kp || ldw % 16 || act < 0 || act > 3 ||
+  if (M <= 0 || N <= 0 || K <= 0 || K > 131071 || ldw < kp || ldw % 16 || act < 0 || act > 3 ||
       (act == ACT_GEGLU && (N % 2 || res)))
     return -1;
   LinArgs p{(const int8_t*)x, (const int8_t*)w, (const float*)sx, (const float*)sw, (const uint16_t*)b,
@@ -798,16 +804,14 @@ ARB_API int arb_linear_int8(const void* x, long ldx, const void* sx, const void*
   if (ldw >= (1L << 22)) return -1;                               // 31-bit offsets in a tile
   if (sx == nullptr && !gamma && arb_linear_int8_few(x, ldx, M, K)) {
     const uint16_t* x16 = (const uint16_t*)x;
-#define FEW(EL, GLU)                                       \
-  if (M == 1) launch_direct<EL, GLU, 1>(p, stream, x16, ldx); \
-  else launch_direct<EL, GLU, 4>(p, stream, x16, ldx)
+#define FEW(EL, GLU) \
+  return M == 1 ? launch_direct<EL, GLU, 1>(p, stream, x16, ldx) : launch_direct<EL, GLU, 4>(p, stream, x16, ldx)
     if (act == ACT_GEGLU) {
-      if (el) { FEW(1, true); } else { FEW(0, true); }
+      if (el) FEW(1, true); else FEW(0, true);
     } else {
-      if (el) { FEW(1, false); } else { FEW(0, false); }
+      if (el) FEW(1, false); else FEW(0, false);
     }
 #undef FEW
-    return (int)hipGetLastError();
   }
   if (sx == nullptr) {
     if (ws == nullptr) return -1;
@@ -819,12 +823,6 @@ ARB_API int arb_linear_int8(const void* x, long ldx, const void* sx, const void*
     p.sx = scale;
   }
   if (p.ldx < kp || p.ldx % 16 || p.ldx >= (1L << 22)) return -1;
-  if (act == ACT_GEGLU) {
-    if (el) launch_linear<1, true>(p, stream);
-    else launch_linear<0, true>(p, stream);
-  } else {
-    if (el) launch_linear<1, false>(p, stream);
-    else launch_linear<0, false>(p, stream);
-  }
-  return (int)hipGetLastError();
+  if (act == ACT_GEGLU) return el ? launch_linear<1, true>(p, stream) : launch_linear<0, true>(p, stream);
+  return el ? launch_linear<1, false>(p, stream) : launch_linear<0, false>(p, stream);
 }

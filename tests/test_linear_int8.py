@@ -185,10 +185,10 @@ def test_linear_int8_activations(device, dtype, act, m, k, n):
 
 @pytest.mark.parametrize("device", DEVICES)
 def test_linear_int8_full_scale_sums(device):
-    """Every product 127 * 127 of one sign: the largest sums, exact to the last bit before the scales."""
-    for k in (16, 1000, 9001, 133000):
-        q = torch.full((3, k), 127, dtype=torch.int8)
-        q[1] = -127
+    """Every product 128 * 128 or -127 * 128: the largest sums, exact to the last bit before the scales."""
+    for k in (16, 1000, 9001, ops.INT8_MAX_K):
+        q = torch.full((3, k), -128, dtype=torch.int8)
+        q[1] = 127
         q[2, 0] = 126
         pad = -k % 16
         store = torch.nn.functional.pad(q, (0, pad)).to(device)
@@ -258,6 +258,8 @@ def test_refusals(device):
                 lambda: ops.linear_int8(x, w, residual=torch.ones(4, 7, dtype=bf, device=device)),
                 lambda: ops.linear_int8(x, w, residual=torch.ones(4, 8, dtype=bf, device=device), act="geglu"),
                 lambda: ops.linear_int8(x, rows(7, 32, 1, device), act="geglu"),
+                lambda: ops.quantize_rows(x[:1, :1].expand(2 ** 31, 1)),
+                lambda: ops.linear_int8(x[:1].expand(2 ** 31, 32), w),
                 lambda: ops.quantize_rows(x[:, :0]), lambda: ops.quantize_rows(torch.ones((), device=device)),
                 lambda: ops.quantize_rows(torch.ones(1, ops.INT8_MAX_K + 1, dtype=bf, device=device)),
                 lambda: ops.ln_quantize_rows(x, x[0, :16], x[0], 1e-5),
@@ -347,7 +349,8 @@ def test_more_rows_than_a_grid_dimension(cuda):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", [None, "geglu"])
-@pytest.mark.parametrize("k,n", [(8, 2), (72, 34), (640, 520), (2048, 96), (8184, 66), (8192, 40), (8200, 40), (77, 30)])
+@pytest.mark.parametrize("k,n", [(8, 2), (72, 34), (640, 520), (2048, 96), (8184, 66), (8192, 40), (8200, 40),
+                                 (77, 30)])
 def test_few_tokens(device, dtype, act, k, n):
     """1 to 17 tokens around every switch of kernels: rows quantised inside the product or apart give the same bits,
     also zero rows, rows with NaN or infinity, and rows cut out of wider ones."""
