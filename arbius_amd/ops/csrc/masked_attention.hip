@@ -36,6 +36,8 @@ ARB_API int arb_masked_attention(const void* q, const void* k, const void* v, vo
   long strides[12], ints[12];
   __builtin_memcpy(strides, dims, sizeof(strides));
   __builtin_memcpy(ints, (const char*)dims + sizeof(strides), sizeof(ints));
+  for (int i = 0; i < 9; ++i)                                     // int counts, a tile past the last key too
+    if (ints[i] > 0x7fffffffL - (i == 7 ? 0 : 1024)) return -1;
   MaskedArgs a;
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v; a.o = (uint16_t*)o;
   a.q_sb = strides[0]; a.q_sn = strides[1]; a.q_sh = strides[2];
@@ -58,7 +60,9 @@ ARB_API int arb_masked_attention(const void* q, const void* k, const void* v, vo
   const KeyPlan kp = key_plan(ints[11], a.H, a.Hkv, a.Nq, a.Nk, a.D);
   a.splits = kp.splits;
   a.wk = kp.wk;
-  if ((long)(a.H / a.Hkv) * a.Nq > 0x7fffffffL - 256 || (rows + 127) * a.splits > 0x7fffffffL) return -1;
+  const long group = (long)(a.H / a.Hkv) * a.Nq, wgs = (group + 127) / 128 * a.Hkv * a.B;
+  // a launch has fewer than 2^32 threads
+  if (group > 0x7fffffffL - 256 || wgs * a.splits >= (1L << 23) || (a.splits > 1 && rows >= (1L << 24))) return -1;
   if (a.splits > 1 && ws == nullptr) return -1;
   a.po = (float*)ws;
   a.pml = a.splits > 1 ? (float2*)((float*)ws + (size_t)a.splits * rows * a.D) : nullptr;

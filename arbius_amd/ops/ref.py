@@ -170,7 +170,8 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
     s = torch.matmul(qf, kf.transpose(-1, -2)) * scale
     if softcap:
         s = softcap * torch.tanh(s / softcap)
-    if slopes is not None:
+    if slopes is not None:               # a position outside the run moved to its edge: the softmax does not see it
+        p = torch.maximum(torch.minimum(p, hi - 1), lo)
         s = s - slopes.float()[None, :, None, None] * (p[..., None] - j).abs().float()[:, None]
     s = torch.where(ok, s, torch.full_like(s, float("-inf")))
     m = s.amax(dim=-1, keepdim=True)

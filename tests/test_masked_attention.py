@@ -100,6 +100,11 @@ def slopes(H):
     return 2.0 ** (-8.0 * torch.arange(1, H + 1, dtype=torch.float32) / H)
 
 
+def spread(n, step):
+    """n offsets, 0 .. step * n, documents of every length from 0 to 3 among them."""
+    return i32([0] + sorted(min(step * n, j * 3 // 2) for j in range(n - 1)) + [step * n])
+
+
 CASES = {
     "plain": dict(shape=(2, 77, 77, 3, 3, 64)),
     "one": dict(shape=(1, 1, 1, 1, 1, 8)),
@@ -141,6 +146,32 @@ CASES = {
                         lengths=i32([12, 402, 2, 700])),
     "long cache, few rows": dict(shape=(1, 1, 5003, 4, 2, 64), causal=True, q_start=5002, slopes=slopes(4)),
     "long cache, short lengths": dict(shape=(2, 1, 5000, 4, 2, 64), lengths=i32([0, 130]), softcap=30.0),
+    # 8 waves, two on the keys
+    "two waves on the keys": dict(shape=(1, 200, 700, 2, 1, 64), causal=True, q_start=500),
+    "two waves, head 96, bias": dict(shape=(1, 130, 640, 2, 2, 96), slopes=slopes(2), lengths=i32([601])),
+    "two waves, head 128, cap": dict(shape=(2, 97, 1100, 1, 1, 128), causal=True, q_start=i32([1000, 3]),
+                                     softcap=30.0),
+    "two waves, head 24, all": dict(shape=(1, 550, 550, 3, 1, 24), causal=True, softcap=10.0, slopes=slopes(3),
+                                    documents=i32([0, 40, 520, 550]), prefix=i32([9, 0, 40])),
+    # key ranges: few of them, more than 64, one that sees nothing
+    "ranges of a few rows": dict(shape=(2, 7, 2000, 4, 2, 64), causal=True, q_start=i32([1993, 300])),
+    "more than 64 ranges": dict(shape=(1, 1, 12000, 2, 2, 32), lengths=i32([11990]), slopes=slopes(2) / 64),
+    "ranges, wide head": dict(shape=(1, 2, 3000, 2, 1, 256), causal=True, q_start=2998, softcap=20.0),
+    "ranges, nothing seen": dict(shape=(3, 1, 3000, 2, 2, 128), lengths=i32([0, -1, 129])),
+    # document searches: empty ones in a row, more than one step of 64 and of 64 x 64 offsets
+    "empty documents in a row": dict(shape=(1, 200, 200, 1, 1, 32), documents=i32([0] + [60] * 150 + [61, 130] +
+                                                                                  [131] * 70 + [200])),
+    "documents of one or two": dict(shape=(1, 1400, 1400, 1, 1, 8), documents=spread(1100, 2)),
+    "thousands of documents": dict(shape=(1, 90, 130, 1, 1, 16), q_start=20, causal=True,
+                                   documents=i32([min(j // 60, 130) for j in range(9000)])),
+    # positions far from the keys, where fp32 holds neither them nor the distances
+    "slopes from far behind": dict(shape=(2, 3, 400, 2, 2, 64), q_start=i32([2 ** 30 + 1, 77777777]),
+                                   slopes=slopes(2) / 8, lengths=i32([400, 130])),
+    "slopes from far ahead": dict(shape=(1, 40, 200, 2, 2, 64), q_start=i32([-2 ** 30]), slopes=slopes(2)),
+    "falling and rising far": dict(shape=(1, 1, 5000, 2, 2, 64), q_start=2 ** 31 - 9,
+                                   slopes=torch.tensor([2.0 ** -4, -2.0 ** -5])),
+    "smallest cap and largest": dict(shape=(1, 50, 90, 2, 2, 64), softcap=2.0 ** -10),
+    "negative scale": dict(shape=(1, 40, 300, 2, 2, 64), scale=-0.2, causal=True, softcap=2.0 ** 10),
     "all": dict(shape=(2, 190, 190, 6, 3, 80), causal=True, documents=i32([3, 90, 180]), prefix=i32([20, 5]),
                 lengths=i32([190, 100]), softcap=10.0, slopes=slopes(6), scale=0.2),
 }
@@ -165,6 +196,9 @@ POISONED = {
     "documents": dict(shape=(1, 210, 210, 2, 1, 64), documents=i32([0, 50, 130, 150])),
     "cache": dict(shape=(3, 1, 4000, 4, 2, 128), causal=True, q_start=i32([0, 77, 3000]), lengths=i32([1, 78, 2001])),
     "causal": dict(shape=(1, 100, 300, 2, 2, 80), causal=True),
+    "two waves on the keys": dict(shape=(1, 150, 800, 1, 1, 128), lengths=i32([707])),
+    "head 160": dict(shape=(1, 40, 200, 1, 1, 160), documents=i32([0, 30, 100])),
+    "head 256": dict(shape=(1, 3, 900, 1, 1, 256), causal=True, q_start=500),
 }
 
 
@@ -204,6 +238,17 @@ def test_a_value_reaches_only_the_queries_that_see_it(device, val):
         assert torch.equal(y[rest], clean[rest])
         got = y[0, hit, 0, 5]
         assert bool(got.isnan().all()) if math.isnan(val) else bool((got == val).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_many_small_weights_next_to_a_large_one(device):
+    """One key of weight 1 and 4000 of 2^-20 each: the small ones keep their bits, also in fp16."""
+    for dt in DTYPES.values():
+        q, k, v = torch.zeros(1, 1, 1, 32), torch.zeros(1, 4001, 1, 32), torch.zeros(1, 4001, 1, 32)
+        q[..., 0], k[:, 1:, :, 0], v[:, 1:, :, 0] = 1.0, -13.8125, 1000.0
+        v[:, 0, :, 1] = 1.0
+        q, k, v = q.to(dt), k.to(dt), v.to(dt)
+        check(run(q, k, v, dict(scale=1.0), device), *definition(q, k, v, dict(scale=1.0)))
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -273,6 +318,8 @@ def test_refusals(device):
                 lambda: att(q[..., :32], k, k), lambda: att(q[:, :, :3], k, k),
                 lambda: att(q, k, k, scale=float("nan")), lambda: att(q, k, k, softcap=0.0),
                 lambda: att(q, k, k, softcap=-1.0), lambda: att(q, k, k, softcap=float("inf")),
+                lambda: att(q, k, k, softcap=1e4), lambda: att(q, k, k, softcap=1e-4), lambda: att(q, k, k, scale=1e7),
+                lambda: att(q[:1].expand(2 ** 31, -1, -1, -1), *2 * (k[:1].expand(2 ** 31, -1, -1, -1),)),
                 lambda: att(q, k, k, q_start=-1), lambda: att(q, k, k, q_start=2 ** 31),
                 lambda: att(q, k, k, lengths=n[:1]), lambda: att(q, k, k, q_start=n[:1]),
                 lambda: att(q, k, k, documents=n[:1]), lambda: att(q, k, k, documents=n[:0]),
