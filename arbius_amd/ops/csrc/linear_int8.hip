@@ -4,7 +4,7 @@
 //   a_r = max_k |x_rk|,  s_r = a_r / 127,  q_rk = rne(127 x_rk / a_r)
 //   y_mn = act( sx_m sw_n sum_k qx_mk qw_nk + b_n + r_mn )
 //
-// The sum is an integer (|sum| <= 127^2 K < 2^31 for every K the host accepts), so it is exact in any
+// The sum is an integer (|sum| <= 128^2 K < 2^31 for every K the host accepts), so it is exact in any
 // order: tiles, k-splits and batch sizes never change a bit of the result.
 #include "common.h"
 
@@ -90,6 +90,12 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
   return v;
 }
 
+// LayerNorm's two roundings that every kernel shares: a row's bits must not depend on the kernel that takes it
+__device__ __forceinline__ float add_square(float sum, float x, float mean) { return fmaf(x - mean, x - mean, sum); }
+__device__ __forceinline__ float normalised(float x, float mean, float rstd, float g, float b) {
+  return fmaf((x - mean) * rstd, g, b);
+}
+
 // One row per T threads, held in registers: V vectors of 8 elements per thread, K <= 8 T V, K % 8 == 0, 16-byte
 // aligned rows.  LN: LayerNorm in fp32 first (two exact passes over the registers), the normalised row not
 // rounded before it is quantised.  Bound by memory: 2 bytes read and 1 written per element in one pass.
@@ -123,7 +129,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint16_t* __re
     for (int i = 0; i < V; ++i)
       if (t + T * i < NV) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += (f[i][e] - mean) * (f[i][e] - mean);
+        for (int e = 0; e < 8; ++e) ss = add_square(ss, f[i][e], mean);
       }
     const float rstd = rsqrtf(row_reduce<T, false>(ss, red) / (float)K + eps);
 #pragma unroll
@@ -133,7 +139,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint16_t* __re
         dec8<EL>(ld16(gamma + 8 * (t + T * i)), g);
         dec8<EL>(ld16(beta + 8 * (t + T * i)), b);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[i][e] = (f[i][e] - mean) * rstd * g[e] + b[e];
+        for (int e = 0; e < 8; ++e) f[i][e] = normalised(f[i][e], mean, rstd, g[e], b[e]);
       }
   }
   float a = 0.f;
@@ -700,6 +706,254 @@ __global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs 
   }
 }
 
+// Short rows (K <= 32 KS), many of them: LayerNorm, quantisation and product in one kernel, x read once and never
+// written in 8 bits.  A wave owns 32 tokens: its lanes l and l + 32 hold the two halves of every 32 bytes of token
+// l & 31 - the B operand's layout - from the 16-bit row to the finished quantised fragments, which stay in registers
+// while the workgroup walks its weight rows, 64 at a time (GLU: 32 values and their 32 gates), through two LDS
+// stages.  The scale of a token is a register of its lanes, so the epilogue runs in the accumulators' layout and only
+// the finished 16-bit channels cross lanes (LDS patch) for 16-byte stores.
+// LN sums are those of quantize_rows_kernel with its 8 (KS 10) or 16 (KS 20) lanes per row, addition by addition.
+template <int EL, bool GLU, bool LN, int KS, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p, const uint16_t* __restrict__ x16,
+                                                                      long ldx16, const uint16_t* __restrict__ gamma,
+                                                                      const uint16_t* __restrict__ beta, float eps,
+                                                                      int splits) {
+  constexpr int BM = 32 * NW, OW = GLU ? 32 : 64, STAGE = KS * 32 * 64, NDMA = 2 * KS / NW, PR = OW + 8;
+  constexpr int LPR = OW / 8, RPI = 64 / LPR, NST = 32 / RPI;     // stores: lanes per row, rows each, per chunk
+  static_assert(NW % 4 == 0 && 2 * KS % NW == 0, "one row group per wave");
+  __shared__ __attribute__((aligned(16))) int8_t st0[STAGE];
+  __shared__ __attribute__((aligned(16))) int8_t st1[STAGE];
+  __shared__ __attribute__((aligned(16))) uint16_t patch[NW][32 * PR];
+  __shared__ __attribute__((aligned(16))) float schan[NW][2][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int NO = GLU ? p.N / 2 : p.N, chunks = (NO + OW - 1) / OW;
+  const int lin = xcd_remap(blockIdx.x, (p.M + BM - 1) / BM * splits), rt = lin / splits, sp = lin - rt * splits;
+  const int per = (chunks + splits - 1) / splits, c0 = min(chunks, sp * per), c1 = min(chunks, c0 + per);
+  const int m0 = rt * BM + 32 * wave, m = m0 + col;
+  const int kp = (p.K + 15) & ~15;
+
+  const uint16_t* xr = x16 + (long)min(m, p.M - 1) * ldx16 + 16 * half;
+  uint4 xv[KS][2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      xv[s][j] = 32 * s + 16 * half + 8 * j < p.K ? ld16(xr + 32 * s + 8 * j) : make_uint4(0, 0, 0, 0);
+
+  // weight stage: 64-byte K tiles of 64 rows, 16-byte chunks XOR-swizzled by the row; instruction q = wave + NW i
+  // fills rows 16 (q & 3) .. + 15 of K tile q >> 2
+  const int wrow = 16 * (wave & 3) + (lane >> 2), kc = 16 * ((lane & 3) ^ ((wrow >> 2) & 3));
+  const bool gate = GLU && (wave & 2);
+  const int orow = gate ? wrow - 32 : wrow;                       // of the chunk's value / gate rows
+  auto issue = [&](int c, int8_t* dst) __attribute__((always_inline)) {
+    const int8_t* base = p.w + ((gate ? NO : 0) + (long)c * OW) * p.ldw;
+    const unsigned off = c * OW + orow < NO ? (unsigned)(orow * (int)p.ldw + kc) : kZeros;
+#pragma unroll
+    for (int i = 0; i < NDMA; ++i) {
+      const int k0 = 64 * ((wave >> 2) + NW / 4 * i);
+      dma_i8(base, dst + 1024 * (wave + NW * i), k0 + kc < kp ? off : kZeros, k0);
+    }
+  };
+  // channel `lane` of a chunk (GLU: values, then gates): read a chunk ahead
+  float csw = 0.f;
+  uint32_t cb = 0;
+  auto channels = [&](int c) __attribute__((always_inline)) {
+    const int n = min(c * OW + (GLU ? col : lane), NO - 1), row = GLU && half ? NO + n : n;
+    csw = p.sw[row];
+    cb = p.b ? p.b[row] : 0;
+  };
+
+  // ---- the wave's tokens: LayerNorm statistics, largest value, fragments.  Every pass decodes the row again: held as
+  // floats between the passes (what hipcc does by itself) it would not fit the registers
+  unsigned gat = 32 * half;
+  auto packed = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        asm volatile("" : "+v"(xv[s][j].x), "+v"(xv[s][j].y), "+v"(xv[s][j].z), "+v"(xv[s][j].w));
+    asm volatile("" : "+v"(gat));                                 // gamma and beta are read again too
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  float mean = 0.f, rstd = 1.f;
+  if constexpr (LN) {
+    for (int v = tid; v < 8 * KS; v += 64 * NW) {                 // gamma, then beta, zeros behind the row
+      const int k = 8 * (v % (4 * KS));
+      st16(st1 + 16 * v, k < p.K ? ld16((v < 4 * KS ? gamma : beta) + k) : make_uint4(0, 0, 0, 0));
+    }
+    __syncthreads();
+    constexpr int G = KS == 10 ? 2 : 4;                           // 4 G lanes per row there: accumulators of 2 G here
+    auto total = [&](float (&t)[2 * G]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int o = G; o > 1; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < o; ++u) t[u] += t[u + o];
+      return sum_xor32(t[0]) + sum_xor32(t[1]);
+    };
+    float t[2 * G], f[8];
+#pragma unroll
+    for (int u = 0; u < 2 * G; ++u) t[u] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        dec8<EL>(xv[s][j], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[2 * (s % G) + j] += f[e];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    mean = total(t) / (float)p.K;
+    packed();
+#pragma unroll
+    for (int u = 0; u < 2 * G; ++u) t[u] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        dec8<EL>(xv[s][j], f);
+        const bool in = 32 * s + 16 * half + 8 * j < p.K;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          t[2 * (s % G) + j] = add_square(t[2 * (s % G) + j], in ? f[e] : mean, mean);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    rstd = rsqrtf(total(t) / (float)p.K + eps);
+    packed();
+  }
+  auto values = [&](int s, int j, float (&f)[8]) __attribute__((always_inline)) {
+    dec8<EL>(xv[s][j], f);
+    if constexpr (LN) {
+      const int8_t* at = st1 + gat + 64 * s + 16 * j;
+      float g[8], b[8];
+      dec8<EL>(ld16(at), g);
+      dec8<EL>(ld16(at + 64 * KS), b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = normalised(f[e], mean, rstd, g[e], b[e]);
+    }
+  };
+  float a = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float f[8];
+      values(s, j, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        bad |= f[e] != f[e];
+        a = fmaxf(a, fabsf(f[e]));
+      }
+    }
+    if (LN || s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+  }
+  a = max_xor32(bad ? INFINITY : a);
+  packed();
+  float sx, inv, up;
+  quant_scale(a, sx, inv, up);
+  uint4 xq[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    float f[8], g[8];
+    values(s, 0, f);
+    values(s, 1, g);
+    const uint2 u = quant8(f, inv, up), v = quant8(g, inv, up);
+    xq[s] = inv != 0.f ? make_uint4(u.x, u.y, v.x, v.y) : make_uint4(0, 0, 0, 0);
+    if (LN || s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // ---- the workgroup's weight rows
+  const int sw0 = col * 64 + 16 * (half ^ ((col >> 2) & 3)), sw1 = col * 64 + 16 * ((2 + half) ^ ((col >> 2) & 3));
+  uint16_t* const pt = patch[wave];
+  float* const sc = schan[wave][0];
+  auto put_channels = [&]() __attribute__((always_inline)) {      // (a wave's own LDS: in order, no barrier)
+    sc[lane] = csw;
+    sc[64 + lane] = dec16<EL>(cb);
+  };
+  auto chunk = [&](int c, const int8_t* st) __attribute__((always_inline)) {
+    i32x16 acc[2] = {(i32x16){}, (i32x16){}};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        acc[t] = mma_i8(ld16(st + 4096 * (s >> 1) + 2048 * t + (s & 1 ? sw1 : sw0)), xq[s], acc[t]);
+    const int n0 = c * OW;
+#pragma unroll
+    for (int t = 0; t < (GLU ? 1 : 2); ++t)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int ch = 32 * t + 2 * i + 4 * half;                 // channels ch .. + 3 of the chunk
+        const f32x4 w = *reinterpret_cast<const f32x4*>(sc + ch), b = *reinterpret_cast<const f32x4*>(sc + 64 + ch);
+        float f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = fmaf((float)acc[t][i + e] * sx, w[e], b[e]);
+        if constexpr (GLU) {
+          const f32x4 gw = *reinterpret_cast<const f32x4*>(sc + 32 + ch);
+          const f32x4 gb = *reinterpret_cast<const f32x4*>(sc + 96 + ch);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] *= gelu_f(fmaf((float)acc[1][i + e] * sx, gw[e], gb[e]));
+        } else {
+          if (p.res && m < p.M && n0 + ch < NO) {
+            const uint2 r = *reinterpret_cast<const uint2*>(p.res + (long)m * NO + n0 + ch);
+            f[0] += dec16<EL>(r.x & 0xffffu);
+            f[1] += dec16<EL>(r.x >> 16);
+            f[2] += dec16<EL>(r.y & 0xffffu);
+            f[3] += dec16<EL>(r.y >> 16);
+          }
+          if (p.act == ACT_GELU) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = gelu_f(f[e]);
+          } else if (p.act == ACT_QUICK_GELU) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] *= __builtin_amdgcn_rcpf(1.f + fast_exp(-1.702f * f[e]));
+          }
+        }
+        *reinterpret_cast<uint2*>(pt + col * PR + ch) = make_uint2(enc16x2<EL>(f[0], f[1]), enc16x2<EL>(f[2], f[3]));
+      }
+    put_channels();                                               // the next chunk's: does not wait for the stores
+    const int r = lane / LPR, cc = lane % LPR * 8;
+    uint16_t* y = p.y + (long)(m0 + r) * NO + n0 + cc;
+    if (m0 + 32 <= p.M && n0 + OW <= NO) {                        // uniform
+      uint4 v[NST];
+#pragma unroll
+      for (int i = 0; i < NST; ++i) v[i] = ld16(pt + (r + RPI * i) * PR + cc);
+#pragma unroll
+      for (int i = 0; i < NST; ++i) st16(y + (long)RPI * i * NO, v[i]);
+      asm volatile("" ::: "memory");
+      wait_dma<NST>();                                            // all but these stores: the other stage has arrived
+    } else {
+#pragma unroll
+      for (int i = 0; i < NST; ++i)
+        if (m0 + r + RPI * i < p.M && n0 + cc < NO) st16(y + (long)RPI * i * NO, ld16(pt + (r + RPI * i) * PR + cc));
+      asm volatile("" ::: "memory");
+      wait_dma<0>();
+    }
+    __builtin_amdgcn_s_barrier();
+  };
+  if (c0 >= c1) return;
+  issue(c0, st0);
+  channels(c0);
+  put_channels();
+  wait_dma<0>();
+  __builtin_amdgcn_s_barrier();
+  for (int c = c0; c < c1; c += 2) {
+    if (c + 1 < c1) {
+      issue(c + 1, st1);
+      channels(c + 1);
+    }
+    chunk(c, st0);
+    if (c + 1 >= c1) break;
+    if (c + 2 < c1) {
+      issue(c + 2, st0);
+      channels(c + 2);
+    }
+    chunk(c + 1, st1);
+  }
+}
+
 template <int EL, bool LN>
 static int launch_quantize(const uint16_t* x, long ldx, const uint16_t* g, const uint16_t* b, float eps, int8_t* q,
                             int ldq, float* scale, long rows, int K, hipStream_t stream) {
@@ -782,6 +1036,21 @@ static int launch_linear(const LinArgs& p, hipStream_t s) {
   return launch_tiles<EL, GLU, 64, 128, 2, WN, 4>(p, s);
 }
 
+template <int EL, bool GLU, bool LN>
+static int launch_rows(const LinArgs& p, const uint16_t* x, long ldx, const uint16_t* g, const uint16_t* b, float eps,
+                       hipStream_t s) {
+  const bool wide = p.K > 320;
+  const int chunks = GLU ? (p.N / 2 + 31) / 32 : (p.N + 63) / 64, bm = wide ? 256 : 128;
+  const long tiles = (p.M + bm - 1L) / bm;
+  const int splits = (int)max(1L, min((wide ? 256 : 512) / tiles, (long)chunks));
+  if (tiles * splits * 2 * bm >= (1L << 32)) return -1;           // a launch has fewer threads
+  const dim3 grid((unsigned)(tiles * splits));
+  if constexpr (!LN)
+    if (wide) linear_int8_rows_kernel<EL, GLU, LN, 20, 8><<<grid, 512, 0, s>>>(p, x, ldx, g, b, eps, splits);
+  if (!wide) linear_int8_rows_kernel<EL, GLU, LN, 10, 4><<<grid, 256, 0, s>>>(p, x, ldx, g, b, eps, splits);
+  return (int)hipGetLastError();
+}
+
 // Whether a product of 16-bit rows without LayerNorm quantises them itself: up to 4 tokens.  (Behind a LayerNorm the
 // sums would run in another order than for longer batches.)
 ARB_API int arb_linear_int8_few(const void* x, long ldx, int M, int K) {
@@ -812,6 +1081,19 @@ ARB_API int arb_linear_int8(const void* x, long ldx, const void* sx, const void*
       if (el) FEW(1, false); else FEW(0, false);
     }
 #undef FEW
+  }
+  if (sx == nullptr && p.vec && K <= (gamma ? 320 : 640) && M >= 8192 && K % 8 == 0 && ldx % 8 == 0 &&
+      ((size_t)x | (size_t)gamma | (size_t)beta) % 16 == 0) {
+    const uint16_t *xp = (const uint16_t*)x, *g = (const uint16_t*)gamma, *be = (const uint16_t*)beta;
+#define ROWS(EL, GLU)                                                            \
+  return g ? launch_rows<EL, GLU, true>(p, xp, ldx, g, be, eps, stream)          \
+           : launch_rows<EL, GLU, false>(p, xp, ldx, g, be, eps, stream)
+    if (act == ACT_GEGLU) {
+      if (el) ROWS(1, true); else ROWS(0, true);
+    } else {
+      if (el) ROWS(1, false); else ROWS(0, false);
+    }
+#undef ROWS
   }
   if (sx == nullptr) {
     if (ws == nullptr) return -1;

@@ -408,3 +408,51 @@ def test_few_tokens_in_a_graph(cuda):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, ops.linear_int8(ops.quantize_rows(x), w))
+
+
+# ------------------------------------------------------------------ many short rows
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ln", [False, True])
+@pytest.mark.parametrize("act", [None, "gelu", "quick_gelu", "geglu"])
+@pytest.mark.parametrize("m,k,n", [(8192, 320, 192), (8193, 312, 80), (8417, 64, 1040), (8448, 8, 16), (8221, 640, 400),
+                                   (8300, 328, 48), (8192, 576, 2064), (40000, 160, 32)])
+def test_many_short_rows(device, dtype, ln, act, m, k, n):
+    """Rows quantised (and normalised) inside the product: bit for bit the two operators apart, with zero rows, rows
+    with NaN or infinity, rows cut out of wider ones."""
+    dt = DTYPES[dtype]
+    if device == "cpu":
+        m = m % 100 + 8
+    x = randn(64, k + 8, seed=k, dtype=dt, device=device).repeat(-(-m // 64), 1)[:m, 8:]
+    x[:, ::5] *= torch.linspace(0.1, 3, m, device=device)[:, None].to(dt)
+    x[3], x[m - 2], x[5, k - 1], x[m - 1, 0] = 0, 0, float("nan"), float("inf")
+    gamma, beta = (1 + 0.1 * randn(k, seed=2)).to(x), (0.1 * randn(k, seed=3)).to(x)
+    w, b = rows(n, k, 4, device, dt), randn(n, seed=5, dtype=dt, device=device)
+    res = randn(m, n, seed=6, dtype=dt, device=device)
+    for bias, r in ((b, None), (None, None if act == "geglu" else res)):
+        if ln:
+            y = ops.ln_linear_int8(x, gamma, beta, 1e-5, w, bias, residual=r, act=act)
+            q = ops.ln_quantize_rows(x, gamma, beta, 1e-5)
+        else:
+            y, q = ops.linear_int8(x, w, bias, residual=r, act=act), ops.quantize_rows(x)
+        want = ops.linear_int8(q, w, bias, residual=r, act=act)
+        bad = torch.zeros(m, dtype=torch.bool, device=device)
+        bad[5] = bad[m - 1] = True
+        assert torch.equal(y.isnan().all(dim=1), bad) and torch.equal(y[~bad], want[~bad])
+
+
+@pytest.mark.gpu
+def test_many_short_rows_in_a_graph(cuda):
+    x, w = randn(8200, 320, seed=1, dtype=torch.bfloat16, device=cuda), rows(384, 320, 2, cuda)
+    gamma, beta = torch.ones(320, device=cuda).to(x), torch.zeros(320, device=cuda).to(x)
+    ops.ln_linear_int8(x, gamma, beta, 1e-5, w)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.ln_linear_int8(x, gamma, beta, 1e-5, w)
+        z = ops.linear_int8(x, w, act="geglu")
+    for step in range(4):
+        x.copy_(randn(8200, 320, seed=5 + step, dtype=torch.bfloat16))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.linear_int8(ops.ln_quantize_rows(x, gamma, beta, 1e-5), w))
+        assert torch.equal(z, ops.linear_int8(ops.quantize_rows(x), w, act="geglu"))
