@@ -90,15 +90,55 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
   return v;
 }
 
-// LayerNorm's two roundings that every kernel shares: a row's bits must not depend on the kernel that takes it
-__device__ __forceinline__ float add_square(float sum, float x, float mean) { return fmaf(x - mean, x - mean, sum); }
-__device__ __forceinline__ float normalised(float x, float mean, float rstd, float g, float b) {
-  return fmaf((x - mean) * rstd, g, b);
+// A row on T threads, V vectors of 8 elements each (thread t: vectors t, t + T, ..; zeros behind the row): its values
+// (LN: of LayerNorm in fp32, two exact passes over the registers, the normalised row not rounded before it is
+// quantised), scale and reciprocal.
+template <int EL, bool LN, int T, int V>
+__device__ __forceinline__ void row_values(const uint4 (&raw)[V], int t, int K, const uint16_t* __restrict__ gamma,
+                                           const uint16_t* __restrict__ beta, float eps, float* red,
+                                           float (&f)[V][8], float& s, float& inv, float& up) {
+  const int NV = K >> 3;
+#pragma unroll
+  for (int i = 0; i < V; ++i) dec8<EL>(raw[i], f[i]);
+  if constexpr (LN) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += f[i][e];
+    const float mean = row_reduce<T, false>(sum, red) / (float)K;
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (t + T * i < NV) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(f[i][e] - mean, f[i][e] - mean, ss);
+      }
+    const float rstd = rsqrtf(row_reduce<T, false>(ss, red) / (float)K + eps);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (t + T * i < NV) {
+        float g[8], b[8];
+        dec8<EL>(ld16(gamma + 8 * (t + T * i)), g);
+        dec8<EL>(ld16(beta + 8 * (t + T * i)), b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] = fmaf((f[i][e] - mean) * rstd, g[e], b[e]);
+      }
+  }
+  float a = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      bad |= f[i][e] != f[i][e];
+      a = fmaxf(a, fabsf(f[i][e]));
+    }
+  quant_scale(row_reduce<T, true>(bad ? INFINITY : a, red), s, inv, up);
 }
 
-// One row per T threads, held in registers: V vectors of 8 elements per thread, K <= 8 T V, K % 8 == 0, 16-byte
-// aligned rows.  LN: LayerNorm in fp32 first (two exact passes over the registers), the normalised row not
-// rounded before it is quantised.  Bound by memory: 2 bytes read and 1 written per element in one pass.
+// One row per T threads: K <= 8 T V, K % 8 == 0, 16-byte aligned rows.  Bound by memory: 2 bytes read and 1 written
+// per element in one pass.
 template <int EL, bool LN, int T, int V>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint16_t* __restrict__ x, long ldx,
                                                             const uint16_t* __restrict__ gamma,
@@ -111,49 +151,14 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint16_t* __re
   if (T < 256 && row >= rows) return;
   const uint16_t* xr = x + row * ldx;
   const int NV = K >> 3;
-  float f[V][8];
+  uint4 raw[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = t + T * i;
-    dec8<EL>(v < NV ? ld16(xr + 8 * v) : make_uint4(0, 0, 0, 0), f[i]);
+    raw[i] = v < NV ? ld16(xr + 8 * v) : make_uint4(0, 0, 0, 0);
   }
-  if constexpr (LN) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s += f[i][e];
-    const float mean = row_reduce<T, false>(s, red) / (float)K;
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (t + T * i < NV) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = add_square(ss, f[i][e], mean);
-      }
-    const float rstd = rsqrtf(row_reduce<T, false>(ss, red) / (float)K + eps);
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (t + T * i < NV) {
-        float g[8], b[8];
-        dec8<EL>(ld16(gamma + 8 * (t + T * i)), g);
-        dec8<EL>(ld16(beta + 8 * (t + T * i)), b);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[i][e] = normalised(f[i][e], mean, rstd, g[e], b[e]);
-      }
-  }
-  float a = 0.f;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bad |= f[i][e] != f[i][e];
-      a = fmaxf(a, fabsf(f[i][e]));
-    }
-  a = row_reduce<T, true>(bad ? INFINITY : a, red);
-  float s, inv, up;
-  quant_scale(a, s, inv, up);
+  float f[V][8], s, inv, up;
+  row_values<EL, LN, T, V>(raw, t, K, gamma, beta, eps, red, f, s, inv, up);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = t + T * i;
@@ -707,12 +712,11 @@ __global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs 
 }
 
 // Short rows (K <= 32 KS), many of them: LayerNorm, quantisation and product in one kernel, x read once and never
-// written in 8 bits.  A wave owns 32 tokens: its lanes l and l + 32 hold the two halves of every 32 bytes of token
-// l & 31 - the B operand's layout - from the 16-bit row to the finished quantised fragments, which stay in registers
-// while the workgroup walks its weight rows, 64 at a time (GLU: 32 values and their 32 gates), through two LDS
-// stages.  The scale of a token is a register of its lanes, so the epilogue runs in the accumulators' layout and only
+// written in 8 bits.  A wave owns 32 tokens: it quantises them as quantize_rows_kernel does (the same lanes per row,
+// the same bits), 64 / T rows at a time, through LDS into the B operand's layout, and their fragments stay in
+// registers while the workgroup walks its weight rows, 64 at a time (GLU: 32 values and their 32 gates), through two
+// LDS stages.  A token's scale is a register of its lanes, so the epilogue runs in the accumulators' layout and only
 // the finished 16-bit channels cross lanes (LDS patch) for 16-byte stores.
-// LN sums are those of quantize_rows_kernel with its 8 (KS 10) or 16 (KS 20) lanes per row, addition by addition.
 template <int EL, bool GLU, bool LN, int KS, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p, const uint16_t* __restrict__ x16,
                                                                       long ldx16, const uint16_t* __restrict__ gamma,
@@ -725,6 +729,7 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
   __shared__ __attribute__((aligned(16))) int8_t st1[STAGE];
   __shared__ __attribute__((aligned(16))) uint16_t patch[NW][32 * PR];
   __shared__ __attribute__((aligned(16))) float schan[NW][2][64];
+  __shared__ float stok[NW][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int NO = GLU ? p.N / 2 : p.N, chunks = (NO + OW - 1) / OW;
@@ -732,14 +737,6 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
   const int per = (chunks + splits - 1) / splits, c0 = min(chunks, sp * per), c1 = min(chunks, c0 + per);
   const int m0 = rt * BM + 32 * wave, m = m0 + col;
   const int kp = (p.K + 15) & ~15;
-
-  const uint16_t* xr = x16 + (long)min(m, p.M - 1) * ldx16 + 16 * half;
-  uint4 xv[KS][2];
-#pragma unroll
-  for (int s = 0; s < KS; ++s)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      xv[s][j] = 32 * s + 16 * half + 8 * j < p.K ? ld16(xr + 32 * s + 8 * j) : make_uint4(0, 0, 0, 0);
 
   // weight stage: 64-byte K tiles of 64 rows, 16-byte chunks XOR-swizzled by the row; instruction q = wave + NW i
   // fills rows 16 (q & 3) .. + 15 of K tile q >> 2
@@ -764,106 +761,47 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
     cb = p.b ? p.b[row] : 0;
   };
 
-  // ---- the wave's tokens: LayerNorm statistics, largest value, fragments.  Every pass decodes the row again: held as
-  // floats between the passes (what hipcc does by itself) it would not fit the registers
-  unsigned gat = 32 * half;
-  auto packed = [&]() __attribute__((always_inline)) {
+  if (c0 >= c1) return;
+  // ---- the wave's tokens, RP rows at a time through its part of the weight stages
+  constexpr int T = KS == 10 ? 8 : 16, V = 5, RI = 64 / T, RP = 2 * STAGE / NW / (32 * KS), SWZ = KS == 10 ? 3 : 7;
+  static_assert(8 * T * V == 32 * KS && RP * NW * 32 * KS == 2 * STAGE && 32 % RP == 0 && RP % RI == 0, "passes");
+  int8_t* const mine = (wave < NW / 2 ? st0 : st1) + wave % (NW / 2) * (RP * 32 * KS);
+  const int t = lane % T, NV = p.K >> 3;
+  auto fetch = [&](int r, uint4 (&raw)[V]) __attribute__((always_inline)) {   // row r of the wave's 32
+    const uint16_t* xr = x16 + (long)min(m0 + r, p.M - 1) * ldx16;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        asm volatile("" : "+v"(xv[s][j].x), "+v"(xv[s][j].y), "+v"(xv[s][j].z), "+v"(xv[s][j].w));
-    asm volatile("" : "+v"(gat));                                 // gamma and beta are read again too
-    __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < V; ++i) raw[i] = t + T * i < NV ? ld16(xr + 8 * (t + T * i)) : make_uint4(0, 0, 0, 0);
   };
-  float mean = 0.f, rstd = 1.f;
-  if constexpr (LN) {
-    for (int v = tid; v < 8 * KS; v += 64 * NW) {                 // gamma, then beta, zeros behind the row
-      const int k = 8 * (v % (4 * KS));
-      st16(st1 + 16 * v, k < p.K ? ld16((v < 4 * KS ? gamma : beta) + k) : make_uint4(0, 0, 0, 0));
-    }
-    __syncthreads();
-    constexpr int G = KS == 10 ? 2 : 4;                           // 4 G lanes per row there: accumulators of 2 G here
-    auto total = [&](float (&t)[2 * G]) __attribute__((always_inline)) {
+  auto swz = [](int r) { return SWZ == 3 ? (r >> 2) & 3 : (r >> 1) & 7; };   // 16-byte units of a staged row, by bank
+  uint4 xq[KS], raw[V];
+  fetch(lane / T, raw);
 #pragma unroll
-      for (int o = G; o > 1; o >>= 1)
+  for (int pass = 0; pass < 32 / RP; ++pass) {
+#pragma unroll 1
+    for (int it = 0; it < RP / RI; ++it) {
+      const int r = it * RI + lane / T, next = pass * RP + r + RI;
+      uint4 now[V];
 #pragma unroll
-        for (int u = 0; u < o; ++u) t[u] += t[u + o];
-      return sum_xor32(t[0]) + sum_xor32(t[1]);
-    };
-    float t[2 * G], f[8];
+      for (int i = 0; i < V; ++i) now[i] = raw[i];
+      if (next < 32) fetch(next, raw);
+      float f[V][8], s, inv, up;
+      row_values<EL, LN, T, V>(now, t, p.K, gamma, beta, eps, nullptr, f, s, inv, up);
 #pragma unroll
-    for (int u = 0; u < 2 * G; ++u) t[u] = 0.f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        dec8<EL>(xv[s][j], f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[2 * (s % G) + j] += f[e];
+      for (int i = 0; i < V; ++i) {
+        const int v = t + T * i;
+        *reinterpret_cast<uint2*>(mine + r * (32 * KS) + 16 * ((v >> 1) ^ swz(r)) + 8 * (v & 1)) =
+            v < NV && inv != 0.f ? quant8(f[i], inv, up) : make_uint2(0u, 0u);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if (t == 0) stok[wave][pass * RP + r] = s;
     }
-    mean = total(t) / (float)p.K;
-    packed();
+    if (RP == 32 || col / RP == pass) {
+      const int r = col % RP;
 #pragma unroll
-    for (int u = 0; u < 2 * G; ++u) t[u] = 0.f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        dec8<EL>(xv[s][j], f);
-        const bool in = 32 * s + 16 * half + 8 * j < p.K;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          t[2 * (s % G) + j] = add_square(t[2 * (s % G) + j], in ? f[e] : mean, mean);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      for (int s = 0; s < KS; ++s) xq[s] = ld16(mine + r * (32 * KS) + 16 * ((2 * s + half) ^ swz(r)));
     }
-    rstd = rsqrtf(total(t) / (float)p.K + eps);
-    packed();
   }
-  auto values = [&](int s, int j, float (&f)[8]) __attribute__((always_inline)) {
-    dec8<EL>(xv[s][j], f);
-    if constexpr (LN) {
-      const int8_t* at = st1 + gat + 64 * s + 16 * j;
-      float g[8], b[8];
-      dec8<EL>(ld16(at), g);
-      dec8<EL>(ld16(at + 64 * KS), b);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = normalised(f[e], mean, rstd, g[e], b[e]);
-    }
-  };
-  float a = 0.f;
-  bool bad = false;
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float f[8];
-      values(s, j, f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        bad |= f[e] != f[e];
-        a = fmaxf(a, fabsf(f[e]));
-      }
-    }
-    if (LN || s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-  }
-  a = max_xor32(bad ? INFINITY : a);
-  packed();
-  float sx, inv, up;
-  quant_scale(a, sx, inv, up);
-  uint4 xq[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    float f[8], g[8];
-    values(s, 0, f);
-    values(s, 1, g);
-    const uint2 u = quant8(f, inv, up), v = quant8(g, inv, up);
-    xq[s] = inv != 0.f ? make_uint4(u.x, u.y, v.x, v.y) : make_uint4(0, 0, 0, 0);
-    if (LN || s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-  }
+  const float sx = stok[wave][col];
+  __syncthreads();                                                // the stages are the weight's from here on
 
   // ---- the workgroup's weight rows
   const int sw0 = col * 64 + 16 * (half ^ ((col >> 2) & 3)), sw1 = col * 64 + 16 * ((2 + half) ^ ((col >> 2) & 3));
@@ -873,13 +811,15 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
     sc[lane] = csw;
     sc[64 + lane] = dec16<EL>(cb);
   };
-  auto chunk = [&](int c, const int8_t* st) __attribute__((always_inline)) {
-    i32x16 acc[2] = {(i32x16){}, (i32x16){}};
+  auto product = [&](const int8_t* st, i32x16 (&acc)[2]) __attribute__((always_inline)) {
+    acc[0] = acc[1] = (i32x16){};
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         acc[t] = mma_i8(ld16(st + 4096 * (s >> 1) + 2048 * t + (s & 1 ? sw1 : sw0)), xq[s], acc[t]);
+  };
+  auto finish = [&](int c, const i32x16 (&acc)[2], auto plain) __attribute__((always_inline)) {
     const int n0 = c * OW;
 #pragma unroll
     for (int t = 0; t < (GLU ? 1 : 2); ++t)
@@ -895,7 +835,7 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
           const f32x4 gb = *reinterpret_cast<const f32x4*>(sc + 96 + ch);
 #pragma unroll
           for (int e = 0; e < 4; ++e) f[e] *= gelu_f(fmaf((float)acc[1][i + e] * sx, gw[e], gb[e]));
-        } else {
+        } else if constexpr (decltype(plain)::value == 0) {
           if (p.res && m < p.M && n0 + ch < NO) {
             const uint2 r = *reinterpret_cast<const uint2*>(p.res + (long)m * NO + n0 + ch);
             f[0] += dec16<EL>(r.x & 0xffffu);
@@ -913,6 +853,15 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
         }
         *reinterpret_cast<uint2*>(pt + col * PR + ch) = make_uint2(enc16x2<EL>(f[0], f[1]), enc16x2<EL>(f[2], f[3]));
       }
+    if constexpr (decltype(plain)::value == 1) {                  // fragments four ahead, a product, some epilogue
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, GLU ? 320 / (2 * KS) : 120 / (2 * KS), 0);
+      }
+    }
     put_channels();                                               // the next chunk's: does not wait for the stores
     const int r = lane / LPR, cc = lane % LPR * 8;
     uint16_t* y = p.y + (long)(m0 + r) * NO + n0 + cc;
@@ -931,26 +880,58 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
       asm volatile("" ::: "memory");
       wait_dma<0>();
     }
-    __builtin_amdgcn_s_barrier();
   };
-  if (c0 >= c1) return;
   issue(c0, st0);
   channels(c0);
   put_channels();
   wait_dma<0>();
   __builtin_amdgcn_s_barrier();
-  for (int c = c0; c < c1; c += 2) {
-    if (c + 1 < c1) {
-      issue(c + 1, st1);
-      channels(c + 1);
+  if constexpr (KS == 10) {
+    // Chunk c's product next to chunk c - 1's epilogue, so that matrix cores and VALU work side by side (65536 x 320
+    // -> 960 behind a LayerNorm 54.8 -> 49.9 us; at KS 20, with twice the fragments to hold, it is a tenth slower)
+    auto step = [&](int c, const int8_t* st, int8_t* other, i32x16 (&acc)[2], const i32x16 (&last)[2])
+                    __attribute__((always_inline)) {
+      if (c + 1 < c1) issue(c + 1, other);
+      channels(c);
+      product(st, acc);
+      if (GLU || (!p.res && p.act == ACT_NONE)) finish(c - 1, last, Stage<1>());
+      else finish(c - 1, last, Stage<0>());
+      __builtin_amdgcn_s_barrier();
+    };
+    i32x16 acc0[2], acc1[2];
+    if (c0 + 1 < c1) issue(c0 + 1, st1);
+    product(st0, acc0);
+    wait_dma<0>();
+    __builtin_amdgcn_s_barrier();
+    for (int c = c0 + 1; c < c1; c += 2) {
+      step(c, st1, st0, acc1, acc0);
+      if (c + 1 >= c1) {
+        acc0[0] = acc1[0];
+        acc0[1] = acc1[1];
+        break;
+      }
+      step(c + 1, st0, st1, acc0, acc1);
     }
-    chunk(c, st0);
-    if (c + 1 >= c1) break;
-    if (c + 2 < c1) {
-      issue(c + 2, st0);
-      channels(c + 2);
+    finish(c1 - 1, acc0, Stage<0>());
+  } else {
+    i32x16 acc[2];
+    for (int c = c0; c < c1; c += 2) {
+      if (c + 1 < c1) {
+        issue(c + 1, st1);
+        channels(c + 1);
+      }
+      product(st0, acc);
+      finish(c, acc, Stage<0>());
+      __builtin_amdgcn_s_barrier();
+      if (c + 1 >= c1) break;
+      if (c + 2 < c1) {
+        issue(c + 2, st0);
+        channels(c + 2);
+      }
+      product(st1, acc);
+      finish(c + 1, acc, Stage<0>());
+      __builtin_amdgcn_s_barrier();
     }
-    chunk(c + 1, st1);
   }
 }
 
@@ -1045,9 +1026,8 @@ static int launch_rows(const LinArgs& p, const uint16_t* x, long ldx, const uint
   const int splits = (int)max(1L, min((wide ? 256 : 512) / tiles, (long)chunks));
   if (tiles * splits * 2 * bm >= (1L << 32)) return -1;           // a launch has fewer threads
   const dim3 grid((unsigned)(tiles * splits));
-  if constexpr (!LN)
-    if (wide) linear_int8_rows_kernel<EL, GLU, LN, 20, 8><<<grid, 512, 0, s>>>(p, x, ldx, g, b, eps, splits);
-  if (!wide) linear_int8_rows_kernel<EL, GLU, LN, 10, 4><<<grid, 256, 0, s>>>(p, x, ldx, g, b, eps, splits);
+  if (wide) linear_int8_rows_kernel<EL, GLU, LN, 20, 8><<<grid, 512, 0, s>>>(p, x, ldx, g, b, eps, splits);
+  else linear_int8_rows_kernel<EL, GLU, LN, 10, 4><<<grid, 256, 0, s>>>(p, x, ldx, g, b, eps, splits);
   return (int)hipGetLastError();
 }
 
@@ -1082,7 +1062,14 @@ ARB_API int arb_linear_int8(const void* x, long ldx, const void* sx, const void*
     }
 #undef FEW
   }
-  if (sx == nullptr && p.vec && K <= (gamma ? 320 : 640) && M >= 8192 && K % 8 == 0 && ldx % 8 == 0 &&
+  // Many short rows: one kernel.  Measured against the quantisation and the product apart, us:
+  //                       8192 rows   16384   32768   65536
+  //   320 -> 2560 geglu   28.6/36.4 43.3/54.6 71.8/92.1 124/173      640 -> 5120 geglu  52.6/64.0 87.7/106 156/200
+  //   320 -> 1280 gelu          -   36.9/49.8 58.8/76.5 100/128      512 -> 2048 gelu          -  56.4/57.4 95.2/105
+  //   320 -> 960 (LN)           -   25.9/23.9 33.1/39.7 49.9/69.1    640 -> 1920               -  44.3/43.1 67.1/77.5
+  // (4096 rows: 22.4/19.3 and 36.7/40.9 with geglu; the quantising prologue has too few rows to hide behind)
+  const int many = act == ACT_GEGLU ? 8192 : act == ACT_NONE ? 32768 : 16384;
+  if (sx == nullptr && p.vec && K <= 640 && M >= many && K % 8 == 0 && ldx % 8 == 0 &&
       ((size_t)x | (size_t)gamma | (size_t)beta) % 16 == 0) {
     const uint16_t *xp = (const uint16_t*)x, *g = (const uint16_t*)gamma, *be = (const uint16_t*)beta;
 #define ROWS(EL, GLU)                                                            \

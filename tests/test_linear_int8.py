@@ -415,8 +415,9 @@ def test_few_tokens_in_a_graph(cuda):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("ln", [False, True])
 @pytest.mark.parametrize("act", [None, "gelu", "quick_gelu", "geglu"])
-@pytest.mark.parametrize("m,k,n", [(8192, 320, 192), (8193, 312, 80), (8417, 64, 1040), (8448, 8, 16), (8221, 640, 400),
-                                   (8300, 328, 48), (8192, 576, 2064), (40000, 160, 32)])
+@pytest.mark.parametrize("m,k,n", [(8192, 320, 192), (32769, 312, 80), (32800, 64, 1040), (32900, 8, 16),
+                                   (33221, 640, 400), (32768, 328, 48), (32768, 576, 2064), (40000, 160, 32),
+                                   (32790, 320, 1984)])
 def test_many_short_rows(device, dtype, ln, act, m, k, n):
     """Rows quantised (and normalised) inside the product: bit for bit the two operators apart, with zero rows, rows
     with NaN or infinity, rows cut out of wider ones."""
@@ -443,7 +444,7 @@ def test_many_short_rows(device, dtype, ln, act, m, k, n):
 
 @pytest.mark.gpu
 def test_many_short_rows_in_a_graph(cuda):
-    x, w = randn(8200, 320, seed=1, dtype=torch.bfloat16, device=cuda), rows(384, 320, 2, cuda)
+    x, w = randn(32800, 320, seed=1, dtype=torch.bfloat16, device=cuda), rows(384, 320, 2, cuda)
     gamma, beta = torch.ones(320, device=cuda).to(x), torch.zeros(320, device=cuda).to(x)
     ops.ln_linear_int8(x, gamma, beta, 1e-5, w)
     g = torch.cuda.CUDAGraph()
@@ -451,7 +452,7 @@ def test_many_short_rows_in_a_graph(cuda):
         y = ops.ln_linear_int8(x, gamma, beta, 1e-5, w)
         z = ops.linear_int8(x, w, act="geglu")
     for step in range(4):
-        x.copy_(randn(8200, 320, seed=5 + step, dtype=torch.bfloat16))
+        x.copy_(randn(32800, 320, seed=5 + step, dtype=torch.bfloat16))
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, ops.linear_int8(ops.ln_quantize_rows(x, gamma, beta, 1e-5), w))
