@@ -1209,7 +1209,8 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
         if sd != 1 or (sb | sn | sh) % 8 or t.data_ptr() % 16:
             raise ValueError("masked_attention: last dim must be contiguous, strides/base 16B aligned")
     # keys that share memory (a token stride below D) or lie 8 MiB apart are out of the tile loads' addressing
-    k, v = (t if D <= t.stride(1) < 1 << 22 else t.contiguous() for t in (k, v))
+    k, v = (t if D <= t.stride(1) < 1 << 22 or Nk == 1 else t.contiguous() for t in (k, v))
+    kn, vn = (k.stride(1), v.stride(1)) if Nk > 1 else (D, D)     # one key: its stride may be anything
     o = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
     if not o.numel():
         return o
@@ -1221,9 +1222,9 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
     plan_b = plan_b or B
     wsb = _masked_workspace(B, plan_b, H, Hkv, Nq, Nk, D)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
-    ints = _MASKED_INTS.pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3], B, H, Hkv, Nq, Nk, D,
-                             causal, 0 if starts else q_start, 0 if documents is None else documents.shape[-1] - 1,
-                             docs_sb, prefix_sb, plan_b)
+    ints = _MASKED_INTS.pack(*q.stride()[:3], k.stride(0), kn, k.stride(2), v.stride(0), vn, v.stride(2),
+                             *o.stride()[:3], B, H, Hkv, Nq, Nk, D, causal, 0 if starts else q_start,
+                             0 if documents is None else documents.shape[-1] - 1, docs_sb, prefix_sb, plan_b)
     _check(_launch(q, _fn("arb_masked_attention"), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ints,
                    _ptr(q_start if starts else None), _ptr(lengths), _ptr(documents), _ptr(prefix), _ptr(slopes),
                    _ptr(ws), scale, softcap or 0.0, el), "masked_attention")

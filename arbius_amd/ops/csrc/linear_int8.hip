@@ -138,7 +138,8 @@ __device__ __forceinline__ void row_values(const uint4 (&raw)[V], int t, int K, 
 }
 
 // One row per T threads: K <= 8 T V, K % 8 == 0, 16-byte aligned rows.  Bound by memory: 2 bytes read and 1 written
-// per element in one pass.
+// per element in one pass (16384 x 8192 in 84 us, 4.8 TB/s; LayerNorm 65536 x 320 in 17 us, 3.7 TB/s; 1232 x 4096 in
+// 4.6 us, where the launch counts).
 template <int EL, bool LN, int T, int V>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint16_t* __restrict__ x, long ldx,
                                                             const uint16_t* __restrict__ gamma,
@@ -410,6 +411,9 @@ __device__ __forceinline__ void put_strip(const i32x16 (&acc)[TN][TM], int b, in
 // patch, so that a lane stores (and loads residuals) 8 channels wide with their scales in registers.
 // GLU: 32-row groups of the W tile alternate value rows and gate rows of the same channels, so both
 // halves of an output meet in one lane.
+// Bound by the matrix cores from 256 x 256 tiles on (16384 x 8192 x 8192: 937 us, 2346 Top/s; a library product of that
+// kind 2138), by LDS reads and the latency of a K step where a CU has one 64 x 128 tile (1232 x 4096 -> 1024: 14.4 us,
+// 717 Top/s).
 template <int EL, bool GLU, int BM, int BN, int WM, int WN, int NS>
 __global__ void __launch_bounds__(64 * WM * WN, 1) linear_int8_kernel(LinArgs p) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
@@ -573,7 +577,9 @@ __device__ __forceinline__ uint4 load_i8(const int8_t* base, unsigned off, int k
 // MR > 0 (at most MR tokens, K <= 8192): x comes in 16 bits and every workgroup quantises it for itself, into LDS,
 // while its weights are on their way - a few KB from the L2 instead of a launch.  The quantisation is exact, so
 // this gives the bits of quantize_rows.
-// Bound by the read of the weight: 1 x 2048 -> 8192 in 6.2 us, 2.7 TB/s (8.3 with the quantisation launched apart).
+// Bound by the read of the weight and the latency of one pass over it: 1 x 2048 -> 8192 in 7.1 us with the weight in
+// memory, 2.4 TB/s, in 5.2 with it in the caches (quantisation launched apart: 8.8 and 6.5).  4 tokens: 8.9 (9.0), and
+// one launch less for the host; more are quantised apart.
 template <int EL, bool GLU, int TN, int KW, int MR>
 __global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs p, const uint16_t* __restrict__ x16,
                                                                         long ldx16) {
@@ -717,6 +723,8 @@ __global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs 
 // registers while the workgroup walks its weight rows, 64 at a time (GLU: 32 values and their 32 gates), through two
 // LDS stages.  A token's scale is a register of its lanes, so the epilogue runs in the accumulators' layout and only
 // the finished 16-bit channels cross lanes (LDS patch) for 16-byte stores.
+// Bound by the VALU (quantisation, scales, GELU) next to the write of y: LayerNorm 65536 x 320 -> 960 in 49.9 us (3.4
+// TB/s of x and y; apart 69.1), 16384 x 640 -> 5120 geglu in 87.7 us (1.2 Pop/s; apart 105.7).
 template <int EL, bool GLU, bool LN, int KS, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p, const uint16_t* __restrict__ x16,
                                                                       long ldx16, const uint16_t* __restrict__ gamma,

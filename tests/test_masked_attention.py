@@ -287,6 +287,28 @@ def test_strided_views(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_token_strides_of_any_size(device):
+    """Keys 8 MiB apart, a single key whose token stride is that or nothing, keys that are all the same memory."""
+    q = randn(1, 3, 2, 64, seed=1, dtype=torch.bfloat16).to(device)
+    far = torch.zeros(2 * (1 << 22) + 256, dtype=torch.bfloat16, device=device)
+    for n, stride in ((3, 1 << 22), (1, 1 << 23), (1, 0), (5, 0), (9, 8)):
+        k = far.as_strided((1, n, 2, 64), (128, stride, 64, 1))
+        v = far.as_strided((1, n, 2, 64), (128, stride, 64, 1), 64)
+        far[:1 << 14] = randn(1 << 14, seed=n).to(far)
+        far[(1 << 23):] = randn(256, seed=n + 1).to(far)
+        got, o = ops.masked_attention(q, k, v), dict(causal=False)
+        check(got, *definition(q.cpu(), k.cpu().clone(), v.cpu().clone(), o))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_scale_of_zero(device):
+    q, k, v = (randn(2, 40, 2, 64, seed=s, dtype=torch.float16) for s in (1, 2, 3))
+    for o in (dict(scale=0.0, causal=True), dict(scale=0.0, softcap=3.0, lengths=i32([40, 7]))):
+        got = run(q, k, v, o, device)
+        check(got, *definition(q, k, v, dict(o, scale=1e-30)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_batch_rows_do_not_touch_each_other(device):
     q, k, v = (randn(8, 100, 4, 64, seed=s, dtype=torch.bfloat16).to(device) for s in (1, 2, 3))
     n = i32([100, 3, 77, 64, 65, 1, 50, 99]).to(device)
