@@ -91,10 +91,13 @@ class CLIPTextEncoder(nn.Module):
         """n prompts of any lengths packed end to end, no padding: ids [T] int64, offsets int32 [n + 1]
         (prompt t is ids[offsets[t]:offsets[t + 1]], ending with its EOS) -> (hidden [T, width], pooled
         EOS features [n, width]).  What ``forward`` computes for each prompt alone, up to rounding (the
-        attention walks other key tiles)."""
-        x = self.tok(ids) + self.pos.weight[packed_positions(ids, offsets)[0]]
-        x = x[None]
+        attention walks other key tiles).  The features of an empty prompt, and of one longer than the
+        position table, are NaN."""
+        pos, outside = packed_positions(ids, offsets, self.pos.weight.shape[0])
+        x = (self.tok(ids) + self.pos.weight[pos]).masked_fill(outside[:, None], float("nan"))[None]
         for layer in self.layers[:len(self.layers) - self.cfg.skip_last]:
             x = layer(x, documents=offsets)
         x = self.final_ln(x)[0]
-        return x, x[offsets[1:].long() - 1]
+        last = offsets[1:].long() - 1
+        lost = (last < offsets[:-1]) | (offsets[:-1] < 0) | (last >= x.shape[0])
+        return x, x[last.clamp(0, x.shape[0] - 1)].masked_fill(lost[:, None], float("nan"))

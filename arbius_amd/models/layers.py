@@ -141,12 +141,15 @@ def init_weights(module: nn.Module, seed: int = 0) -> nn.Module:
     return module
 
 
-def packed_positions(ids, offsets):
-    """(position in its prompt, index of its prompt) of every token of prompts packed end to end (offsets
-    int32 [n + 1], the prompts' first tokens and the end)."""
+def packed_positions(ids, offsets, longest):
+    """Of every token of prompts packed end to end (offsets int32 [n + 1], the prompts' first tokens and the end): its
+    position in its prompt, and whether it is outside - of every prompt, or past the ``longest`` tokens a model
+    has positions for (the position is clamped then; nothing here waits for the device)."""
     at = torch.arange(ids.shape[0], device=ids.device, dtype=torch.int32)
     doc = torch.searchsorted(offsets, at, right=True) - 1
-    return at - offsets[doc], doc
+    pos = at - offsets[doc]
+    outside = (doc < 0) | (doc >= offsets.shape[0] - 1) | (pos < 0) | (pos >= longest)
+    return pos.clamp(0, longest - 1), outside
 
 
 def int8_linears(module: nn.Module, on: bool = True) -> int:

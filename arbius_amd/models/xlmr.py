@@ -146,14 +146,22 @@ class MCLIPText(nn.Module):
     def forward_packed(self, ids, offsets):
         """n sequences of any lengths packed end to end, no padding: ids [T] int64, offsets int32 [n + 1] ->
         (full [T, W], pooled [n, proj]): what ``forward`` computes for the real tokens of each sequence,
-        up to rounding."""
-        pos, _ = packed_positions(ids, offsets)
+        up to rounding.  The features of an empty sequence, and of one longer than the position table, are
+        NaN; a sequence whose tokens are not finite keeps that to itself."""
+        pos, outside = packed_positions(ids, offsets, self.pos.weight.shape[0] - 2)
         x = self.tok(ids) + self.pos(pos + 2) + self.tok_type.weight[0]
-        x = self.ln(x)[None]
+        x = self.ln(x.masked_fill(outside[:, None], float("nan")))[None]
         for layer in self.layers:
             x = layer(x, None, documents=offsets)
-        x = x[0]
-        off = offsets.long()
-        total = torch.nn.functional.pad(x.double().cumsum(dim=0), (0, 0, 1, 0))[off]     # fixed order, no atomics
-        pooled = (total[1:] - total[:-1]) / (off[1:] - off[:-1])[:, None]
+        x, off = x[0], offsets.long()
+        at = off.clamp(0, x.shape[0])
+        fine = x.isfinite().all(dim=1, keepdim=True)
+
+        def sums(t):                                                            # fixed order, no atomics
+            total = torch.nn.functional.pad(t.double().cumsum(dim=0), (0, 0, 1, 0))[at]
+            return total[1:] - total[:-1]
+
+        n = (off[1:] - off[:-1])[:, None]
+        lost = (n <= 0) | (sums(~fine) > 0) | ((at != off)[1:] | (at != off)[:-1])[:, None]
+        pooled = (sums(x.masked_fill(~fine, 0.0)) / n).masked_fill(lost, float("nan"))
         return x, self.proj(pooled.to(x.dtype))

@@ -457,3 +457,29 @@ def test_packed_prompts_through_the_text_towers(device, int8):
             tol = 2e-4 if dt == torch.float32 and not int8 else 0.03
             assert (part.float() - one[0].float()).norm() <= tol * one[0].float().norm()
             assert (pooled[t].float() - pool[0].float()).norm() <= tol * pool[0].float().norm()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("int8", [False, True])
+def test_prompts_that_do_not_fit_are_marked(device, int8):
+    """Empty prompts, prompts longer than the position table, tokens before and behind all prompts, offsets past the
+    tokens: NaN for those, the others' features untouched, and no index leaves its table."""
+    dt = torch.bfloat16 if device == "cuda" else torch.float32
+    off = i32([4, 30, 30, 150, 160, 171, 400]).to(device)               # 26 tokens, none, 120, 10, 11, too many
+    ids = torch.randint(3, 900, (200,), generator=torch.Generator().manual_seed(1)).to(device)
+    clip = layers.init_weights(CLIPTextEncoder(CLIPTextConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256)), 1)
+    xlmr = layers.init_weights(MCLIPText(XLMRConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256, max_pos=100,
+                                                    proj_dim=64)), 2)
+    good = torch.tensor([True, False, False, True, True, False])
+    for model in (clip, xlmr):
+        model.to(device=device, dtype=dt).eval()
+        if int8:
+            layers.int8_linears(model)
+        full, pooled = model.forward_packed(ids, off)
+        assert torch.equal(pooled.isnan().all(dim=1).cpu(), ~good) and bool(pooled[good].isfinite().all())
+        assert bool(full[:4].isnan().all()) and bool(full[4:30].isfinite().all())
+        fit = i32([0, 26, 36, 47]).to(device)
+        alone = model.forward_packed(torch.cat([ids[4:30], ids[150:171]]), fit)[1]
+        # the same prompts at other places of other key tiles: two layers of roundings, an 8-bit step where one flips
+        assert (pooled[good].float() - alone.float()).norm() <= (2e-4 if device == "cpu" and not int8 else 0.03) * \
+            alone.float().norm()
