@@ -431,6 +431,27 @@ def test_streams_and_graph_replays(cuda, nq, nk):
             assert torch.equal(graphs[i][1], ops.masked_attention(q[i], k, v, **o))
 
 
+@pytest.mark.gpu
+def test_calls_at_once_on_two_streams(cuda):
+    """Split attention and 8-bit linears in flight together: each call has its own workspace."""
+    q, k, v = (randn(2, n, h, 64, seed=s, dtype=torch.bfloat16).to(cuda) for s, n, h in ((1, 1, 4), (2, 6000, 2),
+                                                                                         (3, 6000, 2)))
+    x, w = (randn(n, 640, seed=n, dtype=torch.bfloat16).to(cuda) for n in (700, 640))
+    w = ops.quantize_rows(w)
+    starts = [dict(causal=True, q_start=n) for n in (5999, 3000)]
+    want = [ops.masked_attention(q, k, v, **o) for o in starts] + [ops.linear_int8(x, w), ops.linear_int8(x[:3], w)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for step in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append((ops.masked_attention(q, k, v, **starts[i]), ops.linear_int8(x[:3] if i else x, w)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, y in got[i]:
+            assert torch.equal(a, want[i]) and torch.equal(y, want[2 + i])
+
+
 # ------------------------------------------------------------------ as the text towers use it
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("int8", [False, True])
