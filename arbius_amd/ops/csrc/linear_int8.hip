@@ -243,6 +243,12 @@ template <int N>
 __device__ __forceinline__ void wait_dma() {                      // at most N of this wave's loads still in flight
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70 | 0xF00);
 }
+// Every LDS read of this wave has its data, then the workgroup meets: whoever refills a stage behind this barrier finds
+// no read of it under way (a read's own wait may stand behind the barrier, in front of the product that uses it).
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);                             // lgkmcnt 0; DMA counted elsewhere
+  __builtin_amdgcn_s_barrier();
+}
 template <int V>
 struct Stage {
   static constexpr int value = V;
@@ -893,7 +899,7 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
   channels(c0);
   put_channels();
   wait_dma<0>();
-  __builtin_amdgcn_s_barrier();
+  lds_barrier();
   if constexpr (KS == 10) {
     // Chunk c's product next to chunk c - 1's epilogue, so that matrix cores and VALU work side by side (65536 x 320
     // -> 960 behind a LayerNorm 54.8 -> 49.9 us; at KS 20, with twice the fragments to hold, it is a tenth slower)
@@ -904,13 +910,13 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
       product(st, acc);
       if (GLU || (!p.res && p.act == ACT_NONE)) finish(c - 1, last, Stage<1>());
       else finish(c - 1, last, Stage<0>());
-      __builtin_amdgcn_s_barrier();
+      lds_barrier();
     };
     i32x16 acc0[2], acc1[2];
     if (c0 + 1 < c1) issue(c0 + 1, st1);
     product(st0, acc0);
     wait_dma<0>();
-    __builtin_amdgcn_s_barrier();
+    lds_barrier();
     for (int c = c0 + 1; c < c1; c += 2) {
       step(c, st1, st0, acc1, acc0);
       if (c + 1 >= c1) {
@@ -930,7 +936,7 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
       }
       product(st0, acc);
       finish(c, acc, Stage<0>());
-      __builtin_amdgcn_s_barrier();
+      lds_barrier();
       if (c + 1 >= c1) break;
       if (c + 2 < c1) {
         issue(c + 2, st0);
@@ -938,7 +944,7 @@ __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p,
       }
       product(st1, acc);
       finish(c + 1, acc, Stage<0>());
-      __builtin_amdgcn_s_barrier();
+      lds_barrier();
     }
   }
 }
