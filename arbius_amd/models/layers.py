@@ -157,13 +157,17 @@ def int8_linears(module: nn.Module, on: bool = True) -> int:
     channel; activations per token as they come) or, with ``on=False``, in their own type again.  An
     operator's choice per deployment: other bytes than the 16-bit layers, so never for a registered model
     whose solutions other nodes verify.  Returns the number of layers.  Call it again after the weights
-    change; linears used through their bare ``weight`` (fused or hoisted projections) stay as they are."""
-    n = 0
-    for m in module.modules():
-        if isinstance(m, Linear):
-            m.int8 = ops.quantize_rows(m.weight) if on else None
-            n += 1
-    return n
+    change; linears used through their bare ``weight`` (fused or hoisted projections) stay as they are.
+
+    All weights are quantised before the first layer changes, and their kernels have finished: pipeline forks share
+    the layers across threads and streams (``ops.derived_ready``)."""
+    linears = [m for m in module.modules() if isinstance(m, Linear)]
+    forms = [ops.quantize_rows(m.weight) if on else None for m in linears]
+    for q in {f.device: f.q for f in forms if f is not None}.values():
+        ops.derived_ready(q)
+    for m, form in zip(linears, forms):
+        m.int8 = form
+    return len(linears)
 
 
 def timestep_embedding(t, dim, flip_sin_to_cos=True, freq_shift=0.0, max_period=10000):

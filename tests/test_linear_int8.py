@@ -309,6 +309,25 @@ def test_layers_in_8_bits(device):
     assert torch.equal(m(x), before)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_layers_in_8_bits_are_published_when_they_are_ready(device, monkeypatch):
+    """Forks on other streams share the layers: none is switched before the kernels of all have finished, and none
+    where a later one cannot be."""
+    m = layers.init_weights(_Block(), 3).to(device=device, dtype=torch.bfloat16)
+    seen = []
+
+    def ready(t):
+        seen.append((t.device, [lin.int8 for lin in (m.fc1, m.fc2)]))
+    monkeypatch.setattr(ops, "derived_ready", ready)
+    layers.int8_linears(m)
+    assert seen == [(m.fc1.weight.device, [None, None])] and m.fc1.int8 is not None and m.fc2.int8 is not None
+    layers.int8_linears(m, False)
+    m.fc2.weight = nn.Parameter(m.fc2.weight.int(), requires_grad=False)
+    with pytest.raises(TypeError):
+        layers.int8_linears(m)
+    assert m.fc1.int8 is None
+
+
 @pytest.mark.gpu
 def test_streams_and_graph_replays(cuda):
     x = randn(33, 640, seed=1, dtype=torch.bfloat16, device=cuda)
