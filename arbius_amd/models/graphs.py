@@ -16,9 +16,8 @@ from typing import Callable, Sequence
 
 import torch
 
-# Captures are serialised process-wide; "thread_local" capture mode lets other threads keep
-# launching work on their own streams while one thread captures (concurrent task streams).
-CAPTURE_LOCK = threading.Lock()
+from .layers import CAPTURE_LOCK, Int8Uses
+
 # ARB_GRAPH_DEBUG=1: log every capture and every replay whose host call takes > 20 ms (stderr)
 _DEBUG = os.environ.get("ARB_GRAPH_DEBUG", "0") == "1"
 
@@ -109,9 +108,22 @@ def live_table(tensors) -> list:
     return [(t, t.data_ptr(), t.untyped_storage().nbytes()) for t in tensors]
 
 
-def check_live(table) -> None:
+def stale(graph) -> bool:
+    """Whether layers of a captured graph (its ``uses``) have changed between 16 and 8 bits since; waits for its replays
+    then, so that the caller can drop it and capture again."""
+    if graph.uses.current():
+        return False
+    with CAPTURE_LOCK:
+        torch.cuda.synchronize(graph.device)
+    return True
+
+
+def check_live(table, uses) -> None:
     """Before a replay: every captured buffer is still the tensor it was captured on (same address, same
-    storage size).  A replay into a moved or re-sized block would write another tensor's memory."""
+    storage size), every captured layer in the form it had.  A replay into a moved or re-sized block would write
+    another tensor's memory."""
+    if not uses.current():
+        raise RuntimeError("graph captured with layers that have changed between 16 and 8 bits since")
     for t, ptr, nbytes in table:
         if t.data_ptr() != ptr or t.untyped_storage().nbytes() != nbytes:
             raise RuntimeError(f"graph buffer moved: {ptr:#x} -> {t.data_ptr():#x} "
@@ -120,12 +132,12 @@ def check_live(table) -> None:
 
 class GraphedCall:
     def __init__(self, fn: Callable, example_args: Sequence[torch.Tensor], warmup: int = 2):
-        dev = example_args[0].device
+        self.device = dev = example_args[0].device
         self.fn = fn
         self.inputs = [a.detach().clone() for a in example_args]
         if _DEBUG:
             _dbg(f"capture {getattr(fn, '__qualname__', fn)} {[tuple(a.shape) for a in example_args]}")
-        with CAPTURE_LOCK:
+        with CAPTURE_LOCK, Int8Uses() as self.uses:
             s = capture_stream(dev)
             s.wait_stream(torch.cuda.current_stream(dev))
             with torch.cuda.stream(s):
@@ -139,10 +151,10 @@ class GraphedCall:
         self._live = live_table(list(self.inputs) + [o for o in outs if isinstance(o, torch.Tensor)])
 
     def check_live(self):
-        check_live(self._live)
+        check_live(self._live, self.uses)
 
     def __call__(self, *args):
-        check_live(self._live)
+        self.check_live()
         for dst, src in zip(self.inputs, args):
             if src.data_ptr() != dst.data_ptr():
                 dst.copy_(src)
@@ -158,7 +170,8 @@ class GraphedCall:
 
 
 class GraphCache:
-    """Graphs keyed by input shapes (one per resolution / batch)."""
+    """Graphs keyed by input shapes (one per resolution / batch); captured again where layers have changed between 16
+    and 8 bits (``layers.int8_linears``)."""
 
     def __init__(self, fn: Callable, enabled: bool):
         self.fn, self.enabled = fn, enabled
@@ -169,7 +182,7 @@ class GraphCache:
             return self.fn(*args)
         key = tuple(tuple(a.shape) for a in args)
         g = self.graphs.get(key)
-        if g is None:
+        if g is None or stale(g):
             g = self.graphs[key] = GraphedCall(self.fn, args)
         return g(*args)
 

@@ -12,11 +12,42 @@ benchmark runs random-init weights of the real architectures.
 from __future__ import annotations
 
 import math
+import threading
 
 import torch
 import torch.nn as nn
 
 from .. import ops
+
+# Captures are serialised process-wide; "thread_local" capture mode lets other threads keep
+# launching work on their own streams while one thread captures (concurrent task streams).
+CAPTURE_LOCK = threading.RLock()
+_USES = threading.local()        # .log: the Int8Uses entered on this thread
+_SWITCHES = [None]               # another object after every change of a layer between 16 and 8 bits
+
+
+class Int8Uses:
+    """``with Int8Uses() as uses:`` - the form (``Int8Rows``, or None: 16 bits) of every ``Linear`` that this thread runs
+    meanwhile.  A captured graph keeps one: it holds the 8-bit tensors whose addresses the graph replays, and
+    ``current`` tells whether the layers still have the form that was captured."""
+
+    def __init__(self):
+        self.forms, self.seen = {}, _SWITCHES[0]
+
+    def __enter__(self):
+        self.prev, _USES.log = getattr(_USES, "log", None), self.forms
+        return self
+
+    def __exit__(self, *exc):
+        _USES.log = self.prev
+
+    def current(self) -> bool:
+        switches = _SWITCHES[0]
+        if switches is not self.seen:
+            if any(lin.int8 is not form for lin, form in self.forms.values()):
+                return False
+            self.seen = switches
+        return True
 
 
 class Linear(nn.Module):
@@ -27,15 +58,31 @@ class Linear(nn.Module):
         self.cin, self.cout = cin, cout
         self.int8 = None              # ops.Int8Rows of the weight: this linear runs in 8 bits (int8_linears)
 
+    @property
+    def int8(self):
+        return self._int8
+
+    @int8.setter
+    def int8(self, rows):
+        self._int8, _SWITCHES[0] = rows, object()
+
     def reset(self, gen):
         bound = 1.0 / math.sqrt(self.cin)
         self.weight.data.uniform_(-bound, bound, generator=gen)
         if self.bias is not None:
             self.bias.data.uniform_(-bound, bound, generator=gen)
 
+    def form(self):
+        """The ``Int8Rows`` this layer runs on, None in 16 bits; noted for the capture under way on this thread."""
+        int8, log = self._int8, getattr(_USES, "log", None)
+        if log is not None:
+            log[id(self), id(int8)] = self, int8
+        return int8
+
     def forward(self, x, residual=None, act=None):
-        if self.int8 is not None:
-            return ops.linear_int8(x, self.int8, self.bias, residual=residual, act=act)
+        int8 = self.form()
+        if int8 is not None:
+            return ops.linear_int8(x, int8, self.bias, residual=residual, act=act)
         return ops.linear(x, self.weight, self.bias, residual=residual, act=act)
 
     def forward_norm(self, x, norm):
@@ -107,15 +154,16 @@ class LayerNorm(nn.Module):
 
     def linear(self, x, lin: "Linear", residual=None, act=None):
         """act(lin(self(x))) with this LayerNorm (and the activation) folded into the GEMM (ops.ln_linear)."""
-        if lin.int8 is not None:
-            return ops.ln_linear_int8(x, self.weight, self.bias, self.eps, lin.int8, lin.bias, residual=residual,
-                                      act=act)
+        int8 = lin.form()
+        if int8 is not None:
+            return ops.ln_linear_int8(x, self.weight, self.bias, self.eps, int8, lin.bias, residual=residual, act=act)
         return ops.ln_linear(x, self.weight, self.bias, self.eps, lin.weight, lin.bias, residual=residual, act=act)
 
     def linear_geglu(self, x, lin: "Linear"):
         """GEGLU projection of self(x) with this LayerNorm folded in (ops.ln_linear_geglu)."""
-        if lin.int8 is not None:
-            return ops.ln_linear_int8(x, self.weight, self.bias, self.eps, lin.int8, lin.bias, act="geglu")
+        int8 = lin.form()
+        if int8 is not None:
+            return ops.ln_linear_int8(x, self.weight, self.bias, self.eps, int8, lin.bias, act="geglu")
         return ops.ln_linear_geglu(x, self.weight, self.bias, self.eps, lin.weight, lin.bias)
 
 
@@ -160,13 +208,22 @@ def int8_linears(module: nn.Module, on: bool = True) -> int:
     change; linears used through their bare ``weight`` (fused or hoisted projections) stay as they are.
 
     All weights are quantised before the first layer changes, and their kernels have finished: pipeline forks share
-    the layers across threads and streams (``ops.derived_ready``)."""
+    the layers across threads and streams (``ops.derived_ready``).  Pipelines capture their graphs again at the next
+    call.  Call it while none is solving: 8-bit weights that it replaces are given back once what the GPUs were
+    doing is done."""
     linears = [m for m in module.modules() if isinstance(m, Linear)]
     forms = [ops.quantize_rows(m.weight) if on else None for m in linears]
     for q in {f.device: f.q for f in forms if f is not None}.values():
         ops.derived_ready(q)
+    old = {}
     for m, form in zip(linears, forms):
+        if m.int8 is not None:
+            old.setdefault(m.int8.device, []).append(m.int8)
         m.int8 = form
+    for device in old:                 # read by kernels of any stream so far
+        if device.type == "cuda":
+            with CAPTURE_LOCK:         # a device is not waited for while a thread captures on it
+                torch.cuda.synchronize(device)
     return len(linears)
 
 

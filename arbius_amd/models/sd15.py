@@ -25,7 +25,7 @@ from .. import ops
 from ..utils.trace import span
 from ..utils.progress import beat
 from .clip_text import CLIPTextConfig, CLIPTextEncoder
-from .graphs import CAPTURE_LOCK, GraphCache, PipelineBase, capture_stream, check_live, live_table
+from .graphs import CAPTURE_LOCK, GraphCache, Int8Uses, PipelineBase, capture_stream, check_live, live_table, stale
 from .layers import init_weights
 from .schedulers import GroupSampler, TaskSampler, make_scheduler
 from .tokenizer import CLIPTokenizer
@@ -53,18 +53,15 @@ class _GraphedUNet:
     at every denoising step (unet2d.cross_kv_mode)."""
 
     def __init__(self, unet, x_shape, ctx, dtype):
-        dev = ctx.device
+        self.device = dev = ctx.device
         self.unet = unet
         self.x = torch.zeros(x_shape, dtype=dtype, device=dev)
         self.t = torch.zeros(1, dtype=torch.float32, device=dev)
         self.ctx = ctx.clone()
         self.kv = {}
         self._ctx_obj = None
-        CAPTURE_LOCK.acquire()
-        try:
+        with CAPTURE_LOCK, Int8Uses() as self.uses:
             self._capture(unet, dev)
-        finally:
-            CAPTURE_LOCK.release()
 
     HOIST = os.environ.get("ARBIUS_CROSS_KV_HOIST", "1") != "0"   # A/B switch (same numerics)
 
@@ -94,7 +91,7 @@ class _GraphedUNet:
         self._live = live_table([self.x, self.t, self.ctx, self.out] + list(self.kv.values()))
 
     def __call__(self, x, t, ctx):
-        check_live(self._live)
+        check_live(self._live, self.uses)
         if x.data_ptr() != self.x.data_ptr():       # the sampler writes the static buffer itself
             self.x.copy_(x)
         self.t.fill_(float(t))
@@ -193,7 +190,7 @@ class SD15Pipeline(PipelineBase):
 
     def _graph(self, shape, ctx):
         with ops.plan_batch(2):
-            if shape not in self._graphs:
+            if shape not in self._graphs or stale(self._graphs[shape]):
                 self._graphs[shape] = _GraphedUNet(self.unet, shape, ctx, self.dtype)
             return self._graphs[shape]
 

@@ -328,6 +328,81 @@ def test_layers_in_8_bits_are_published_when_they_are_ready(device, monkeypatch)
     assert m.fc1.int8 is None
 
 
+def test_a_capture_knows_the_forms_it_used():
+    """What a captured graph keeps of the layers it ran: the 8-bit weights themselves, and whether they still are the
+    layers' weights."""
+    m, other = (layers.init_weights(_Block(), s) for s in (3, 4))
+    x = randn(3, 96, seed=6)
+
+    def capture():
+        with layers.Int8Uses() as uses:
+            m(x)
+        return uses
+    a = capture()
+    assert set(a.forms.values()) == {(m.fc1, None), (m.fc2, None)} and a.current()
+    layers.int8_linears(other)                               # not its layers
+    assert a.current()
+    layers.int8_linears(m.fc2)
+    assert not a.current()
+    b = capture()
+    assert b.current() and (m.fc2, m.fc2.int8) in b.forms.values()
+    layers.int8_linears(m.fc2)                               # quantised again: other tensors
+    assert not b.current() and not a.current()
+    m.fc2.int8 = None
+    assert a.current() and not b.current()
+    m(x)                                                     # outside of a capture nothing is noted
+    assert len(a.forms) == 2
+
+
+@pytest.mark.gpu
+def test_captured_graphs_follow_the_layers(cuda):
+    """Switched on, quantised again after a weight change and off: pipelines and their forks, with graphs captured
+    before, answer as the eager model does, whatever was allocated where the old 8-bit weights were."""
+    from arbius_amd.models.registry import build_pipeline
+    pipe = build_pipeline("anythingv3", device=cuda, use_graphs=True)
+    fork, eager = pipe.fork(), pipe.fork()
+    eager.use_graphs = False
+    eager._reset_graphs()
+    kw = dict(prompt="a lake", width=128, height=128, num_inference_steps=2, scheduler="DPMSolverMultistep", seed=7)
+    images, kept = [], []
+
+    def solve():
+        want = eager(**kw)
+        kept.append([torch.full((1 << 20,), 85, dtype=torch.uint8, device=cuda) for _ in range(64)])
+        for p in (pipe, fork, pipe):
+            assert (p(**kw) == want).all()
+        images.append(want)
+    solve()
+    assert sum(layers.int8_linears(m) for m in (pipe.unet, pipe.text)) > 150
+    solve()
+    with torch.no_grad():
+        for layer in pipe.text.layers:
+            layer.fc2.weight.mul_(0.5)
+    layers.int8_linears(pipe.text)
+    solve()
+    for m in (pipe.unet, pipe.text):
+        layers.int8_linears(m, False)
+    solve()
+    assert all((a != b).any() for i, a in enumerate(images) for b in images[:i])
+
+
+@pytest.mark.gpu
+def test_a_graph_of_other_forms_is_refused(cuda):
+    from arbius_amd.models.graphs import GraphCache, GraphedCall
+    m = layers.init_weights(_Block(), 3).to(device=cuda, dtype=torch.bfloat16)
+    x = randn(5, 96, seed=6, dtype=torch.bfloat16, device=cuda)
+    cache, want = GraphCache(m, True), m(x)
+    old = GraphedCall(m, [x])
+    assert torch.equal(cache(x), want) and torch.equal(old(x), want)
+    layers.int8_linears(m)
+    with pytest.raises(RuntimeError, match="8 bits"):
+        old(x)
+    want8 = m(x)
+    assert torch.equal(cache(x), want8) and not torch.equal(want, want8)
+    layers.int8_linears(m, False)
+    assert torch.equal(cache(x), want) and torch.equal(old(x), want)
+
+
 @pytest.mark.gpu
 def test_streams_and_graph_replays(cuda):
     x = randn(33, 640, seed=1, dtype=torch.bfloat16, device=cuda)
