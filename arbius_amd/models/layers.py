@@ -64,7 +64,12 @@ class Linear(nn.Module):
 
     @int8.setter
     def int8(self, rows):
-        self._int8, _SWITCHES[0] = rows, object()
+        self._int8, self._of = rows, None if rows is None else self._weight()
+        _SWITCHES[0] = object()
+
+    def _weight(self):
+        w = self._parameters["weight"]
+        return w.data_ptr(), w._version, w.dtype
 
     def reset(self, gen):
         bound = 1.0 / math.sqrt(self.cin)
@@ -75,6 +80,10 @@ class Linear(nn.Module):
     def form(self):
         """The ``Int8Rows`` this layer runs on, None in 16 bits; noted for the capture under way on this thread."""
         int8, log = self._int8, getattr(_USES, "log", None)
+        if int8 is not None and self._of != self._weight():        # other values than were quantised
+            int8 = ops.quantize_rows(self.weight)
+            ops.derived_ready(int8.q)
+            self.int8 = int8
         if log is not None:
             log[id(self), id(int8)] = self, int8
         return int8
@@ -204,8 +213,9 @@ def int8_linears(module: nn.Module, on: bool = True) -> int:
     """Run the ``Linear`` layers of ``module`` in 8 bits (``ops.linear_int8``; weights quantised here, once, per output
     channel; activations per token as they come) or, with ``on=False``, in their own type again.  An
     operator's choice per deployment: other bytes than the 16-bit layers, so never for a registered model
-    whose solutions other nodes verify.  Returns the number of layers.  Call it again after the weights
-    change; linears used through their bare ``weight`` (fused or hoisted projections) stay as they are.
+    whose solutions other nodes verify.  Returns the number of layers.  Weights loaded or moved later are
+    quantised again at their next use (changed through ``.data``, which torch does not count, only by another call);
+    linears used through their bare ``weight`` (fused or hoisted projections) stay as they are.
 
     All weights are quantised before the first layer changes, and their kernels have finished: pipeline forks share
     the layers across threads and streams (``ops.derived_ready``).  Pipelines capture their graphs again at the next

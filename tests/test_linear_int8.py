@@ -328,6 +328,31 @@ def test_layers_in_8_bits_are_published_when_they_are_ready(device, monkeypatch)
     assert m.fc1.int8 is None
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_weights_that_change_are_quantised_again(device):
+    """Loaded, changed in place, cast: no layer answers with the 8-bit form of values it no longer has."""
+    m, other = (layers.init_weights(_Block(), s).to(device=device, dtype=torch.bfloat16) for s in (3, 4))
+    x = randn(5, 96, seed=6, dtype=torch.bfloat16, device=device)
+
+    def fresh():
+        again = layers.init_weights(_Block(), 0).to(device=device, dtype=m.fc1.weight.dtype)
+        again.load_state_dict(m.state_dict())
+        layers.int8_linears(again)
+        return again
+    layers.int8_linears(m)
+    first = m(x)
+    m.load_state_dict(other.state_dict())
+    assert torch.equal(m(x), fresh()(x)) and not torch.equal(m(x), first)
+    with torch.no_grad():
+        m.fc2.weight.mul_(2.0)
+    assert torch.equal(m(x), fresh()(x))
+    m.to(torch.float16)
+    assert torch.equal(m(x.half()), fresh()(x.half()))
+    held = m.fc1.int8
+    m(x.half())
+    assert m.fc1.int8 is held
+
+
 def test_a_capture_knows_the_forms_it_used():
     """What a captured graph keeps of the layers it ran: the 8-bit weights themselves, and whether they still are the
     layers' weights."""
