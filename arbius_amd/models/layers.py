@@ -51,11 +51,14 @@ class Int8Uses:
 
 
 class Linear(nn.Module):
-    def __init__(self, cin, cout, bias=True):
+    """``hoisted``: never called itself, its bare weight is read as a part of a batched projection (so it has no 8-bit
+    form)."""
+
+    def __init__(self, cin, cout, bias=True, hoisted=False):
         super().__init__()
         self.weight = nn.Parameter(torch.empty(cout, cin), requires_grad=False)
         self.bias = nn.Parameter(torch.empty(cout), requires_grad=False) if bias else None
-        self.cin, self.cout = cin, cout
+        self.cin, self.cout, self.hoisted = cin, cout, hoisted
         self.int8 = None              # ops.Int8Rows of the weight: this linear runs in 8 bits (int8_linears)
 
     @property
@@ -96,11 +99,21 @@ class Linear(nn.Module):
 
     def forward_norm(self, x, norm):
         """x [B, ..., Cin] with a GroupNorm(+SiLU) prologue from ``norm = (table, silu)`` (table per
-        batch row b): run as a 1x1 implicit-GEMM conv over the [B, 1, N, Cin] view."""
+        batch row b): run as a 1x1 implicit-GEMM conv over the [B, 1, N, Cin] view (8 bits: in a pass of its own)."""
+        int8 = self.form()
+        if int8 is not None:
+            return ops.linear_int8(ops.normed(x, norm), int8, self.bias)
         B, C = x.shape[0], x.shape[-1]
         y = ops.conv2d(x.reshape(B, 1, -1, C), self.weight.view(self.cout, 1, 1, self.cin), self.bias,
                        padding=0, norm=norm)
         return y.view(*x.shape[:-1], self.cout)
+
+    def geglu(self, x):
+        """GEGLU projection (ops.linear_geglu)."""
+        int8 = self.form()
+        if int8 is not None:
+            return ops.linear_int8(x, int8, self.bias, act="geglu")
+        return ops.linear_geglu(x, self.weight, self.bias)
 
 
 class Conv2d(nn.Module):
@@ -215,13 +228,13 @@ def int8_linears(module: nn.Module, on: bool = True) -> int:
     operator's choice per deployment: other bytes than the 16-bit layers, so never for a registered model
     whose solutions other nodes verify.  Returns the number of layers.  Weights loaded or moved later are
     quantised again at their next use (changed through ``.data``, which torch does not count, only by another call);
-    linears used through their bare ``weight`` (fused or hoisted projections) stay as they are.
+    ``hoisted`` layers, of which only the bare weight is used, stay in 16 bits and are not counted.
 
     All weights are quantised before the first layer changes, and their kernels have finished: pipeline forks share
     the layers across threads and streams (``ops.derived_ready``).  Pipelines capture their graphs again at the next
     call.  Call it while none is solving: 8-bit weights that it replaces are given back once what the GPUs were
     doing is done."""
-    linears = [m for m in module.modules() if isinstance(m, Linear)]
+    linears = [m for m in module.modules() if isinstance(m, Linear) and not m.hoisted]
     forms = [ops.quantize_rows(m.weight) if on else None for m in linears]
     for q in {f.device: f.q for f in forms if f is not None}.values():
         ops.derived_ready(q)

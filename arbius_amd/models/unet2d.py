@@ -128,7 +128,7 @@ class FeedForward(nn.Module):
     def forward(self, x, residual, ln=None):
         # GEGLU fused into the projection GEMM's epilogue on the GPU (ops.linear_geglu); ``ln``: the
         # block's LayerNorm of x folded into the same GEMM
-        h = ln.linear_geglu(x, self.proj) if ln is not None else ops.linear_geglu(x, self.proj.weight, self.proj.bias)
+        h = ln.linear_geglu(x, self.proj) if ln is not None else self.proj.geglu(x)
         return self.out(h, residual=residual)
 
 
@@ -170,7 +170,7 @@ class ResBlock(nn.Module):
         super().__init__()
         self.norm1 = GroupNorm(groups, cin, eps, silu=True)
         self.conv1 = Conv2d(cin, cout, 3)
-        self.temb_proj = Linear(temb_dim, cout) if temb_dim else None
+        self.temb_proj = Linear(temb_dim, cout, hoisted=True) if temb_dim else None
         self.norm2 = GroupNorm(groups, cout, eps, silu=True)
         self.conv2 = Conv2d(cout, cout, 3)
         self.shortcut = Conv2d(cin, cout, 1) if cin != cout else None

@@ -304,6 +304,15 @@ def ln_linear_geglu(x, gamma, beta, eps, w, b=None):
     return linear_geglu(layer_norm(x, gamma, beta, eps), w, b)
 
 
+def normed(x, norm):
+    """x [B, ..., C] with a GroupNorm(+SiLU) prologue ``norm`` (``NormSpec`` or (table, silu)) applied, for a consumer
+    that takes no prologue."""
+    if isinstance(norm, NormSpec) and norm.slice_ok():
+        return norm.applied().view(x.shape)
+    table, silu = norm
+    return apply_norm_table(x.reshape(x.shape[0], 1, -1, x.shape[-1]), table, silu).view(x.shape)
+
+
 # --------------------------------------------------------------------------- 8-bit linears
 INT8_MAX_K = 131071          # 128^2 K stays below 2^31: the integer sums never wrap
 

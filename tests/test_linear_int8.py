@@ -329,6 +329,35 @@ def test_layers_in_8_bits_are_published_when_they_are_ready(device, monkeypatch)
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("b,n,c", [(2, 64, 64), (1, 4096, 320)])
+def test_layers_behind_a_group_norm_in_8_bits(device, b, n, c):
+    """GroupNorm then linear, a GEGLU projection without a norm: 8 bits where the layer is switched."""
+    lin = layers.init_weights(nn.ModuleList([layers.Linear(c, 96)]), 3)[0].to(device=device, dtype=torch.bfloat16)
+    norm = layers.init_weights(nn.ModuleList([layers.GroupNorm(8, c)]), 4)[0].to(device=device, dtype=torch.bfloat16)
+    x = (randn(b, n, c, seed=6, device=device) * 2 + 1).to(torch.bfloat16)
+    want, gate = lin.forward_norm(x, norm.table(x, silu=True)), lin.geglu(x)
+    assert layers.int8_linears(lin) == 1
+    got = lin.forward_norm(x, norm.table(x, silu=True))
+    assert torch.equal(got, ops.linear_int8(ops.normed(x, norm.table(x, silu=True)), lin.int8, lin.bias))
+    # both operands off by at most half of 1/127 of their row's largest value
+    assert 0 < (got.float() - want.float()).norm() < 0.03 * want.float().norm()
+    assert torch.equal(lin.geglu(x), ops.linear_int8(x, lin.int8, lin.bias, act="geglu"))
+    assert 0 < (lin.geglu(x).float() - gate.float()).norm() < 2 * 0.03 * gate.float().norm()     # a product of two
+
+
+def test_layers_counted_are_those_that_run_in_8_bits():
+    """Every layer that int8_linears counts runs in 8 bits in a forward pass of the UNet; the time projections, batched
+    through their bare weights, are not among them."""
+    from arbius_amd.models.unet2d import ResBlock, UNet2DCondition, UNetConfig
+    unet = layers.init_weights(UNet2DCondition(UNetConfig.tiny()), 1).eval()
+    count = layers.int8_linears(unet)
+    with layers.Int8Uses() as uses:
+        unet(randn(1, 8, 8, 4, seed=1), torch.tensor([5.0]), randn(1, 7, 32, seed=2))
+    assert count == len(uses.forms) and all(form is not None for _, form in uses.forms.values())
+    assert all(m.temb_proj.int8 is None for m in unet.modules() if isinstance(m, ResBlock))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_weights_that_change_are_quantised_again(device):
     """Loaded, changed in place, cast: no layer answers with the 8-bit form of values it no longer has."""
     m, other = (layers.init_weights(_Block(), s).to(device=device, dtype=torch.bfloat16) for s in (3, 4))
