@@ -240,6 +240,40 @@ def test_a_value_reaches_only_the_queries_that_see_it(device, val):
         assert bool(got.isnan().all()) if math.isnan(val) else bool((got == val).all())
 
 
+SEEN = {   # values that are seen at a weight too small for 32 bits: parts of a split cache, the two-wave plan, one tile run
+    "split cache": dict(shape=(1, 1, 6000, 1, 1, 64), slopes=torch.tensor([0.5])),
+    "split cache, heads": dict(shape=(2, 2, 5000, 4, 2, 128), causal=True, q_start=4000,
+                               slopes=torch.tensor([0.5, 1.0, 2.0, 0.25])),
+    "two waves on the keys": dict(shape=(1, 700, 700, 1, 1, 64), slopes=torch.tensor([2.0])),
+    "one wave, late maximum": dict(shape=(1, 40, 400, 8, 1, 80), causal=True, q_start=360, slopes=torch.full((8,), 2.0)),
+    "head 256": dict(shape=(1, 3, 900, 1, 1, 256), q_start=890, slopes=torch.tensor([1.0])),
+}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", SEEN)
+def test_a_seen_value_shows_at_any_weight(device, dtype, name):
+    """NaN and infinities that a query sees far away, where a distance bias leaves a weight of 0 in 32 bits: NaN, the
+    infinity, or NaN of both signs, in those channels and no others, however the keys are divided."""
+    o = dict(SEEN[name])
+    B, Nq, Nk, H, Hkv, D = o.pop("shape")
+    dt = DTYPES[dtype]
+    q, k, v = randn(B, Nq, H, D, seed=1, dtype=dt), randn(B, Nk, Hkv, D, seed=2, dtype=dt), \
+        randn(B, Nk, Hkv, D, seed=3, dtype=dt)
+    clean = run(q, k, v, o, device).cpu()
+    inf, at = float("inf"), 10 if o.get("q_start") else Nk - 5
+    v[0, at, 0, 5], v[0, at, 0, 9], v[0, at, 0, 12] = float("nan"), inf, -inf
+    v[0, at, 0, 14], v[0, Nk // 2 - 40, 0, 14] = inf, -inf
+    y = run(q, k, v, o, device).cpu()
+    hit, G = y[0, :, :H // Hkv], H // Hkv
+    assert bool(hit[..., 5].isnan().all()) and bool(hit[..., 14].isnan().all())
+    assert bool((hit[..., 9] == inf).all()) and bool((hit[..., 12] == -inf).all())
+    for d in (5, 9, 12, 14):
+        y[0, :, :G, d] = clean[0, :, :G, d]
+    assert torch.equal(y, clean)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_many_small_weights_next_to_a_large_one(device):
     """One key of weight 1 and 4000 of 2^-20 each: the small ones keep their bits, also in fp16."""
