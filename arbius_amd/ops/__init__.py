@@ -810,8 +810,9 @@ def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=No
 
         s_ij = cap tanh(scale q_i.k_j / cap) - slopes[h] |p_i - j|,  o_i = sum_j softmax_j(s_ij) v_j
 
-    over the keys every given mask leaves; a query they leave none gets zeros, and what masked keys and
-    values hold (NaN, infinities, memory never written) does not matter.  p_i = q_start + i is the
+    over the keys every given mask leaves; a query they leave none gets zeros (one whose keys all score -inf gets NaN,
+    0 / 0), and what masked keys and values hold (NaN, infinities, memory never written) does not matter.  A NaN or an
+    infinity in a value that a query sees shows in its result, however small the weight.  p_i = q_start + i is the
     position of query i among the keys.  All optional:
 
     * ``causal``: keys j <= p_i; with ``prefix`` also the first ``prefix`` keys (of the document, if any)

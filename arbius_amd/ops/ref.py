@@ -177,7 +177,7 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
     m = s.amax(dim=-1, keepdim=True)
     e = torch.exp(s - torch.where(m == float("-inf"), torch.zeros_like(m), m))
     total = e.sum(dim=-1, keepdim=True)
-    w = torch.where(total == 0, torch.zeros_like(e), e / total)         # no key (or none but scores of -inf): zeros
+    w = torch.where(ok.any(dim=-1, keepdim=True), e / total, torch.zeros_like(e))       # no key: zeros
     # a masked value never reaches the sum, whatever it holds (0 * NaN would)
     fine = torch.isfinite(vf)
     o = torch.matmul(w, torch.where(fine, vf, torch.zeros_like(vf)))

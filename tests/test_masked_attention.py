@@ -275,6 +275,22 @@ def test_a_seen_value_shows_at_any_weight(device, dtype, name):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nk,heads,start", [(140, 140, 2, 0), (1, 6000, 2, 5990), (700, 700, 1, 0), (2, 300, 4, 290)])
+def test_scores_that_are_all_minus_infinity(device, dtype, nq, nk, heads, start):
+    """Keys, but none with a score above -inf: 0 / 0, where no keys give zeros; one finite score is enough for a row."""
+    dt = DTYPES[dtype]
+    q, k, v = (randn(3, n, heads, 64, seed=s, dtype=dt) for n, s in ((nq, 1), (nk, 2), (nk, 3)))
+    q[..., 0], k[1, :, :, 0] = 1.0, -float("inf")
+    k[2, 1:, :, 0] = -float("inf")
+    o = dict(causal=True, q_start=start, lengths=i32([0, nk, nk]))
+    y = run(q, k, v, o, device).cpu()
+    assert not bool(y[0].any()) and bool(y[1].isnan().all())
+    # (batch row 2: the one key weighs 1)
+    assert torch.equal(y[2], v[2, :1].expand(nq, -1, -1))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_many_small_weights_next_to_a_large_one(device):
     """One key of weight 1 and 4000 of 2^-20 each: the small ones keep their bits, also in fp16."""
     for dt in DTYPES.values():
