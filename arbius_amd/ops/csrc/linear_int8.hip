@@ -73,6 +73,15 @@ __device__ __forceinline__ void dec8(uint4 v, float (&f)[8]) {
     f[2 * i + 1] = dec16<EL>(w[i] >> 16);
   }
 }
+// 8 elements from p (EW: at any element, else 16-byte aligned)
+template <bool EW>
+__device__ __forceinline__ uint4 ld8(const uint16_t* p) {
+  if constexpr (!EW) return ld16(p);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 // sum / maximum over the T threads that share a row (8 .. 64 lanes of a wave, or the block of 256); fixed order
 template <int T, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* red) {
@@ -93,7 +102,7 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
 // A row on T threads, V vectors of 8 elements each (thread t: vectors t, t + T, ..; zeros behind the row): its values
 // (LN: of LayerNorm in fp32, two exact passes over the registers, the normalised row not rounded before it is
 // quantised), scale and reciprocal.
-template <int EL, bool LN, int T, int V>
+template <int EL, bool LN, int T, int V, bool EW = false>
 __device__ __forceinline__ void row_values(const uint4 (&raw)[V], int t, int K, const uint16_t* __restrict__ gamma,
                                            const uint16_t* __restrict__ beta, float eps, float* red,
                                            float (&f)[V][8], float& s, float& inv, float& up) {
@@ -119,8 +128,8 @@ __device__ __forceinline__ void row_values(const uint4 (&raw)[V], int t, int K, 
     for (int i = 0; i < V; ++i)
       if (t + T * i < NV) {
         float g[8], b[8];
-        dec8<EL>(ld16(gamma + 8 * (t + T * i)), g);
-        dec8<EL>(ld16(beta + 8 * (t + T * i)), b);
+        dec8<EL>(ld8<EW>(gamma + 8 * (t + T * i)), g);
+        dec8<EL>(ld8<EW>(beta + 8 * (t + T * i)), b);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[i][e] = fmaf((f[i][e] - mean) * rstd, g[e], b[e]);
       }
@@ -137,10 +146,11 @@ __device__ __forceinline__ void row_values(const uint4 (&raw)[V], int t, int K, 
   quant_scale(row_reduce<T, true>(bad ? INFINITY : a, red), s, inv, up);
 }
 
-// One row per T threads: K <= 8 T V, K % 8 == 0, 16-byte aligned rows.  Bound by memory: 2 bytes read and 1 written
+// One row per T threads: K <= 8 T V, K % 8 == 0, 16-byte aligned rows, gamma and beta (EW: at any element, read by
+// elements - the order of LayerNorm's sums is K's, not the address's).  Bound by memory: 2 bytes read and 1 written
 // per element in one pass (16384 x 8192 in 84 us, 4.8 TB/s; LayerNorm 65536 x 320 in 17 us, 3.7 TB/s; 1232 x 4096 in
 // 4.6 us, where the launch counts).
-template <int EL, bool LN, int T, int V>
+template <int EL, bool LN, int T, int V, bool EW>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint16_t* __restrict__ x, long ldx,
                                                             const uint16_t* __restrict__ gamma,
                                                             const uint16_t* __restrict__ beta, float eps,
@@ -156,10 +166,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint16_t* __re
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = t + T * i;
-    raw[i] = v < NV ? ld16(xr + 8 * v) : make_uint4(0, 0, 0, 0);
+    raw[i] = v < NV ? ld8<EW>(xr + 8 * v) : make_uint4(0, 0, 0, 0);
   }
   float f[V][8], s, inv, up;
-  row_values<EL, LN, T, V>(raw, t, K, gamma, beta, eps, red, f, s, inv, up);
+  row_values<EL, LN, T, V, EW>(raw, t, K, gamma, beta, eps, red, f, s, inv, up);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = t + T * i;
@@ -954,25 +964,41 @@ static int launch_quantize(const uint16_t* x, long ldx, const uint16_t* g, const
                             int ldq, float* scale, long rows, int K, hipStream_t stream) {
   const bool vec = K % 8 == 0 && ldx % 8 == 0 && (size_t)x % 16 == 0 && (size_t)g % 16 == 0 && (size_t)b % 16 == 0;
   const int nv = (ldq + 7) / 8;                                   // vectors a row's threads write
-#define QROWS(T, V)                                                                                            \
-  quantize_rows_kernel<EL, LN, T, V><<<dim3((unsigned)((rows + 256 / T - 1) / (256 / T))), 256, 0, stream>>>(   \
-      x, ldx, g, b, eps, q, ldq, scale, rows, K)
-  // Lanes per row.  LN: by K alone (its sums' order must not depend on the rows of the batch), about 5 vectors a
-  // lane.  Without LN every choice gives the same bits: few rows are spread over whole workgroups.
-  const bool few = !LN && rows < 4096, any = !vec || nv > 2048;
+#define QROWS(T, V)                                                                                              \
+  do {                                                                                                           \
+    const dim3 grid((unsigned)((rows + 256 / T - 1) / (256 / T)));                                               \
+    if (vec) quantize_rows_kernel<EL, LN, T, V, false><<<grid, 256, 0, stream>>>(x, ldx, g, b, eps, q, ldq, scale, \
+                                                                                 rows, K);                       \
+    else quantize_rows_kernel<EL, LN, T, V, LN><<<grid, 256, 0, stream>>>(x, ldx, g, b, eps, q, ldq, scale, rows, \
+                                                                          K);                                    \
+  } while (0)
+  // Lanes per row.  LN: by K alone (its sums' order must not depend on the rows of the batch, nor on where they lie),
+  // about 5 vectors a lane.  Without LN every choice gives the same bits: few rows are spread over whole workgroups.
+  const bool few = !LN && rows < 4096, any = !(vec || (LN && K % 8 == 0)) || nv > 2048;
   // a launch has fewer than 2^32 threads
   if (rows * (any || nv > 320 ? 256 : nv > 160 ? 64 : nv > 80 ? 32 : nv > 40 ? 16 : 8) >= (1L << 32) - 256) return -1;
-  if (any)
+  if (any) {
     quantize_rows_any_kernel<EL, LN><<<dim3((unsigned)rows), 256, 0, stream>>>(x, ldx, g, b, eps, q, ldq, scale, K);
-  else if (nv <= 40 && !few) QROWS(8, 5);
-  else if (nv <= 80 && !few) QROWS(16, 5);
-  else if (nv <= 64) QROWS(64, 1);
-  else if (nv <= 160 && !few) QROWS(32, 5);
-  else if (nv <= 256 && few) QROWS(256, 1);
-  else if (nv <= 320 && !few) QROWS(64, 5);
-  else if (nv <= 512) QROWS(256, 2);
-  else if (nv <= 1024) QROWS(256, 4);
-  else QROWS(256, 8);
+  } else if (few && nv <= 256) {
+    if constexpr (!LN) {
+      if (nv <= 64) QROWS(64, 1);
+      else QROWS(256, 1);
+    }
+  } else if (nv <= 40) {
+    QROWS(8, 5);
+  } else if (nv <= 80) {
+    QROWS(16, 5);
+  } else if (nv <= 160) {
+    QROWS(32, 5);
+  } else if (nv <= 320 && !few) {
+    QROWS(64, 5);
+  } else if (nv <= 512) {
+    QROWS(256, 2);
+  } else if (nv <= 1024) {
+    QROWS(256, 4);
+  } else {
+    QROWS(256, 8);
+  }
 #undef QROWS
   return (int)hipGetLastError();
 }

@@ -533,6 +533,46 @@ def test_layernorm_batch_invariance(device, k):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [8, 312, 320, 328, 640, 1000, 1280, 2048, 2560, 4096, 8192, 16384, 16392, 1001])
+def test_layernorm_order_is_the_lengths_alone(device, dtype, k):
+    """The same rows at an odd base, with a row stride that is no multiple of a vector, or alone, behind gamma and beta at
+    odd bases: the same 8 bits, scales and products."""
+    dt, m = DTYPES[dtype], 200 if k < 4000 else 40
+    x = (randn(m, k, seed=1) * 3 + 0.5).to(dt).to(device)
+    gamma, beta = (1 + 0.1 * randn(k, seed=2)).to(dt).to(device), (0.1 * randn(k, seed=3)).to(dt).to(device)
+    w = rows(40, k, 4, device, dt)
+    odd, apart = torch.empty(m * k + 1, dtype=dt, device=device)[1:].view(m, k), \
+        torch.empty(m, k + 5, dtype=dt, device=device)[:, :k]
+    odd.copy_(x)
+    apart.copy_(x)
+    go, bo = (torch.cat([t[:1], t])[1:] for t in (gamma, beta))
+    want, y = ops.ln_quantize_rows(x, gamma, beta, 1e-5), ops.ln_linear_int8(x, gamma, beta, 1e-5, w)
+    for xs, g, b in ((odd, gamma, beta), (apart, gamma, beta), (x, go, beta), (x, gamma, bo), (apart, go, bo)):
+        got = ops.ln_quantize_rows(xs, g, b, 1e-5)
+        assert torch.equal(got.scale, want.scale) and torch.equal(got.q, want.q)
+        assert torch.equal(ops.ln_linear_int8(xs, g, b, 1e-5, w), y)
+        for i in (0, 7, m - 1):
+            one = ops.ln_quantize_rows(xs[i], g, b, 1e-5)
+            assert torch.equal(one.scale, want.scale[i:i + 1]) and torch.equal(one.q[0], want.q[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [320, 640])
+def test_many_short_rows_behind_a_layernorm_at_any_address(cuda, k):
+    """The kernel of many short rows takes aligned rows only; what it refuses gives the same bits."""
+    m, bf = 33000, torch.bfloat16
+    x = randn(m, k, seed=1, dtype=bf, device=cuda)
+    gamma, beta = (1 + 0.1 * randn(k, seed=2)).to(x), (0.1 * randn(k, seed=3)).to(x)
+    w = rows(136, k, 4, cuda)
+    apart = torch.empty(m, k + 4, dtype=bf, device=cuda)[:, :k]
+    apart.copy_(x)
+    y = ops.ln_linear_int8(x, gamma, beta, 1e-5, w)
+    assert torch.equal(ops.ln_linear_int8(apart, gamma, beta, 1e-5, w), y)
+    assert torch.equal(ops.ln_linear_int8(apart[5], gamma, beta, 1e-5, w), y[5])
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_operands_of_any_alignment(device):
     """Bias and residual cut out of others at odd elements, results whose width is no multiple of a vector."""
     for m, k, n in ((3, 64, 70), (70, 200, 136), (300, 128, 520)):
