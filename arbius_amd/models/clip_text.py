@@ -93,6 +93,9 @@ class CLIPTextEncoder(nn.Module):
         EOS features [n, width]).  What ``forward`` computes for each prompt alone, up to rounding (the
         attention walks other key tiles).  The features of an empty prompt, and of one longer than the
         position table, are NaN."""
+        if not ids.shape[0]:                       # no token, so every prompt is empty (or its tokens are missing)
+            x = self.tok(ids)
+            return x, x.new_full((offsets.shape[0] - 1, x.shape[1]), float("nan"))
         pos, outside = packed_positions(ids, offsets, self.pos.weight.shape[0])
         x = (self.tok(ids) + self.pos.weight[pos]).masked_fill(outside[:, None], float("nan"))[None]
         for layer in self.layers[:len(self.layers) - self.cfg.skip_last]:

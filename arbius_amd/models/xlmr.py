@@ -148,6 +148,9 @@ class MCLIPText(nn.Module):
         (full [T, W], pooled [n, proj]): what ``forward`` computes for the real tokens of each sequence,
         up to rounding.  The features of an empty sequence, and of one longer than the position table, are
         NaN; a sequence whose tokens are not finite keeps that to itself."""
+        if not ids.shape[0]:                       # no token, so every sequence is empty (or its tokens are missing)
+            x = self.tok(ids)
+            return x, x.new_full((offsets.shape[0] - 1, self.proj.cout), float("nan"))
         pos, outside = packed_positions(ids, offsets, self.pos.weight.shape[0] - 2)
         x = self.tok(ids) + self.pos(pos + 2) + self.tok_type.weight[0]
         x = self.ln(x.masked_fill(outside[:, None], float("nan")))[None]

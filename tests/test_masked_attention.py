@@ -554,3 +554,21 @@ def test_prompts_that_do_not_fit_are_marked(device, int8):
         # the same prompts at other places of other key tiles: two layers of roundings, an 8-bit step where one flips
         assert (pooled[good].float() - alone.float()).norm() <= (2e-4 if device == "cpu" and not int8 else 0.03) * \
             alone.float().norm()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("int8", [False, True])
+def test_prompts_without_any_token(device, int8):
+    dt = torch.bfloat16 if device == "cuda" else torch.float32
+    clip = layers.init_weights(CLIPTextEncoder(CLIPTextConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256)), 1)
+    xlmr = layers.init_weights(MCLIPText(XLMRConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256, max_pos=100,
+                                                    proj_dim=64)), 2)
+    none = torch.zeros(0, dtype=torch.long, device=device)
+    for model, width in ((clip, 128), (xlmr, 64)):
+        model.to(device=device, dtype=dt).eval()
+        if int8:
+            layers.int8_linears(model)
+        for off in ([0, 0, 0], [0, 5], [0]):
+            full, pooled = model.forward_packed(none, i32(off).to(device))
+            assert tuple(full.shape) == (0, 128) and full.dtype == pooled.dtype == dt
+            assert tuple(pooled.shape) == (len(off) - 1, width) and bool(pooled.isnan().all())
