@@ -799,7 +799,7 @@ TEMPORAL_MAX_FRAMES = 96     # csrc/temporal_attention.hip keeps <= 96 frames in
 def _index_arg(name, t, like, shapes):
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != like.device:
         raise TypeError(f"masked_attention: {name} must be an int32 tensor on {like.device}")
-    if t.shape not in shapes or t.stride(-1) != 1:
+    if t.shape not in shapes or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f"masked_attention: {name} has shape {tuple(t.shape)} (contiguous {shapes} expected)")
 
 

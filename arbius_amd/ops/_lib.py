@@ -1206,6 +1206,8 @@ def masked_attention(q, k, v, scale, causal, q_start, lengths, prefix, documents
         raise ValueError(f"masked_attention: D={D} not a multiple of 8 up to 256")
     for t in (q, k, v):
         sb, sn, sh, sd = t.stride()
+        if (sb | sn | sh) % 8:                                    # of a size of 1 the stride is never used
+            sb, sn, sh = (st if n > 1 else 0 for n, st in zip(t.shape, (sb, sn, sh)))
         if sd != 1 or (sb | sn | sh) % 8 or t.data_ptr() % 16:
             raise ValueError("masked_attention: last dim must be contiguous, strides/base 16B aligned")
     # keys that share memory (a token stride below D) or lie 8 MiB apart are out of the tile loads' addressing

@@ -351,6 +351,26 @@ def test_token_strides_of_any_size(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_strides_of_single_sizes(device):
+    """One batch row, one token, one head: their strides are never used, so any will do; index tensors of one element
+    cut out of others too."""
+    store = randn(1 << 13, seed=1, dtype=torch.bfloat16).to(device)
+    for b, nq, nk, h, hkv in ((1, 3, 5, 2, 2), (2, 1, 1, 2, 2), (2, 3, 5, 1, 1), (1, 1, 1, 1, 1)):
+        def odd(n, heads, at):
+            full = (512, 64 * heads, 64)
+            strides = [st if size > 1 else st + 3 for size, st in zip((b, n, heads), full)]
+            return store.as_strided((b, n, heads, 64), (*strides, 1), at)
+        q, k, v = odd(nq, h, 0), odd(nk, hkv, 2048), odd(nk, hkv, 4096)
+        got = ops.masked_attention(q, k, v, causal=True)
+        assert torch.equal(got, ops.masked_attention(*(t.clone(memory_format=torch.contiguous_format) for t in (q, k, v)),
+                                                     causal=True))
+    pair = i32([[2, 7], [1, 7]]).to(device)
+    got = ops.masked_attention(*(t[:1] for t in (q, k, v)), causal=True, lengths=pair[1:, 0], q_start=pair[:1, 0],
+                               prefix=pair[:1, 0])
+    assert torch.equal(got, ops.masked_attention(*(t[:1] for t in (q, k, v))))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_scale_of_zero(device):
     q, k, v = (randn(2, 40, 2, 64, seed=s, dtype=torch.float16) for s in (1, 2, 3))
     for o in (dict(scale=0.0, causal=True), dict(scale=0.0, softcap=3.0, lengths=i32([40, 7]))):
