@@ -330,6 +330,8 @@ class Int8Rows:
             raise TypeError("Int8Rows: q int8 and scale fp32 on one device")
         if q.dim() != 2 or scale.shape != q.shape[:1] or not scale.is_contiguous():
             raise ValueError(f"Int8Rows: q {tuple(q.shape)} scale {tuple(scale.shape)} (q [R, K], scale [R])")
+        if torch.is_grad_enabled() and scale.requires_grad:
+            raise RuntimeError("Int8Rows: inference only (no gradients)")
         R, K = q.shape
         if not 1 <= K <= INT8_MAX_K or (shape is not None and (shape[-1] != K or math.prod(shape[:-1]) != R)):
             raise ValueError(f"Int8Rows: q {tuple(q.shape)} for shape {shape} (1 <= K <= {INT8_MAX_K})")
@@ -862,6 +864,8 @@ def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=No
     if slopes is not None and (not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32
                                or slopes.device != device or slopes.shape != (H,) or not slopes.is_contiguous()):
         raise ValueError(f"masked_attention: slopes must be contiguous fp32 [{H}] on {device}")
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("masked_attention: inference only (no gradients)")
     if max(B, H, Nq, ks[1], n) > 2 ** 31 - 1024:
         raise ValueError(f"masked_attention: q {tuple(qs)} k / v {tuple(ks)} pass 2^31")
     args = (q, k, v, scale, bool(causal), q_start, lengths, prefix, documents, softcap, slopes)

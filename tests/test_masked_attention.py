@@ -430,6 +430,18 @@ def test_refusals(device):
         att(q.clone().requires_grad_(), k, k)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_operand_asks_for_a_gradient(device):
+    q, s = torch.ones(1, 3, 4, 64, dtype=torch.bfloat16, device=device), slopes(4).to(device).requires_grad_()
+    with pytest.raises(RuntimeError, match="inference only"):
+        ops.masked_attention(q, q, q, slopes=s)
+    with torch.no_grad():
+        assert torch.equal(ops.masked_attention(q, q, q, slopes=s), ops.masked_attention(q, q, q, slopes=s.detach()))
+    rows = ops.quantize_rows(q[0, 0])
+    with pytest.raises(RuntimeError, match="inference only"):
+        ops.Int8Rows(rows.q, rows.scale.clone().requires_grad_())
+
+
 @pytest.mark.gpu
 def test_gpu_refusals(cuda):
     q = torch.ones(1, 3, 2, 72, dtype=torch.bfloat16, device=cuda)
