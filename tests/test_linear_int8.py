@@ -272,6 +272,38 @@ def test_refusals(device):
         ops.linear_int8(x, w, torch.ones(8, dtype=bf, device=device, requires_grad=True))
 
 
+# The kernel of a size follows from its tiles: 256 x 256 from 256 tiles of that kind on, below that two stages from 512
+# tiles of 64 x 128 on, four stages under it, all above 16 tokens; rows longer than 640 never take the short-row kernel.
+LARGE = {"256 x 256": (4100, 1101, 4099, 4098), "two stages": (2100, 1500, 2050, 2054),
+         "four stages": (517, 1101, 1030, 1030)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,bias,residual", [(None, True, "odd"), (None, False, None), ("gelu", True, "aligned"),
+                                               ("quick_gelu", False, "odd"), ("geglu", True, None)])
+@pytest.mark.parametrize("name", LARGE)
+def test_every_kernel_of_large_products(cuda, dtype, act, bias, residual, name):
+    """Widths that are no multiple of a vector, rows that are none of 16 bytes, residuals at odd elements: the element-wise
+    epilogue of every tile kernel; the same with a width of whole vectors."""
+    dt, (m, k, odd, glu) = DTYPES[dtype], LARGE[name]
+    tiles = lambda bm, bn, n: -(-m // bm) * -(-n // bn)     # noqa: E731
+    for n in ((glu if act == "geglu" else odd), (glu if act == "geglu" else odd) // 16 * 16):
+        want_kernel = ("256 x 256" if tiles(256, 256, n) >= 256 else
+                       "two stages" if tiles(64, 128, n) >= 512 else "four stages")
+        assert want_kernel == name and m > 16 and k > 640
+        x, w = randn(m, k, seed=1, dtype=dt, device=cuda) * 2, rows(n, k, 2, cuda, dt)
+        b = randn(n, seed=3, dtype=dt, device=cuda) if bias else None
+        store = randn(m * n + 8, seed=4, dtype=dt, device=cuda) if residual else None
+        r = None if store is None else store[(1 if residual == "odd" else 8):][:m * n].view(m, n)
+        q = ops.quantize_rows(x)
+        y = ops.linear_int8(x, w, b, residual=r, act=act)
+        want, mag = linear64(q.q, q.scale, w.q, w.scale, b, r, act)
+        over = (y.double() - want).abs() - (torch.finfo(dt).eps / 2 * want.abs() + 2.0 ** -20 * mag + 2.0 ** -25)
+        assert bool((over <= 0).all()), f"n {n}: over the bound by {over.max().item():.3g}"
+        assert torch.equal(ops.linear_int8(q, w, b, residual=r, act=act), y)
+
+
 @pytest.mark.gpu
 def test_gpu_types_refused(cuda):
     with pytest.raises(TypeError):
