@@ -119,6 +119,23 @@ def test_quantize_rows_extremes(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_dequantize_is_half_a_step_off(device, dtype):
+    """Back in the tensor's shape and type: off by half a step of the row (scale / 2) and the type's own rounding, with
+    2^-20 of the row's largest value for the scale's."""
+    x = (randn(3, 5, 77, seed=1) * 4).to(DTYPES[dtype]).to(device)
+    x[1, 2] = 0.0
+    x[2, 4, 3] = float("inf")
+    back = ops.quantize_rows(x).dequantize()
+    assert back.shape == x.shape and back.dtype == x.dtype and bool(back[2, 4].isnan().all())
+    assert not bool(back[1, 2].any())
+    x, back = x.view(15, 77)[:14].double(), back.view(15, 77)[:14].double()
+    top = x.abs().amax(dim=1, keepdim=True)
+    half = torch.finfo(DTYPES[dtype]).eps / 2
+    assert bool(((x - back).abs() <= top * (0.5 / 127 + 2.0 ** -20) * (1 + half) + half * x.abs()).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_quantize_rows_strided_views(device):
     base = randn(3, 5, 4, 96, seed=2, dtype=torch.bfloat16, device=device)
     for x in (base[:, :, 1], base[:, 2], base[1, :, :, 8:72], base[..., 3:80], base.transpose(0, 1), base[..., ::2],

@@ -604,3 +604,30 @@ def test_prompts_without_any_token(device, int8):
             full, pooled = model.forward_packed(none, i32(off).to(device))
             assert tuple(full.shape) == (0, 128) and full.dtype == pooled.dtype == dt
             assert tuple(pooled.shape) == (len(off) - 1, width) and bool(pooled.isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_packed_prompts_in_a_graph(cuda, int8):
+    """One graph over ids and offsets that change between replays, with eager work in between: other prompts, empty ones,
+    one too long, and the same again."""
+    from arbius_amd.models.graphs import GraphedCall
+    clip = layers.init_weights(CLIPTextEncoder(CLIPTextConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256)), 1)
+    xlmr = layers.init_weights(MCLIPText(XLMRConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256, max_pos=100,
+                                                    proj_dim=64)), 2)
+    packs = [[0, 30, 60, 130, 200], [0, 0, 77, 77, 90], [0, 1, 2, 3, 200], [5, 40, 41, 99, 150], [0, 30, 60, 130, 200]]
+    for model in (clip, xlmr):
+        model.to(device=cuda, dtype=torch.bfloat16).eval()
+        if int8:
+            layers.int8_linears(model)
+        ids = [torch.randint(3, 900, (200,), generator=torch.Generator().manual_seed(s)).to(cuda) for s in (1, 2, 3, 4, 1)]
+        with torch.no_grad():
+            want = [tuple(t.clone() for t in model.forward_packed(i, i32(off).to(cuda))) for i, off in zip(ids, packs)]
+            graph = GraphedCall(model.forward_packed, [ids[0], i32(packs[0]).to(cuda)])
+            for _ in range(2):
+                for i, off, (full, pooled) in zip(ids, packs, want):
+                    got = graph(i, i32(off).to(cuda))
+                    torch.cuda.synchronize()
+                    assert torch.equal(got[0].nan_to_num(7.0), full.nan_to_num(7.0))
+                    assert torch.equal(got[1].nan_to_num(7.0), pooled.nan_to_num(7.0))
+                    model.forward_packed(i, i32(off).to(cuda))
