@@ -27,8 +27,8 @@ _SWITCHES = [None]               # another object after every change of a layer 
 
 
 class Int8Uses:
-    """``with Int8Uses() as uses:`` - the form (``Int8Rows``, or None: 16 bits) of every ``Linear`` that this thread runs
-    meanwhile.  A captured graph keeps one: it holds the 8-bit tensors whose addresses the graph replays, and
+    """``with Int8Uses() as uses:`` - the form (``Int8Rows``, or None: 16 bits) of every ``Linear`` that this thread
+    runs meanwhile.  A captured graph keeps one: it holds the 8-bit tensors whose addresses the graph replays, and
     ``current`` tells whether the layers still have the form that was captured."""
 
     def __init__(self):

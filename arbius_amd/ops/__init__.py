@@ -827,6 +827,8 @@ def masked_attention(q, k, v, scale=None, causal=False, q_start=None, lengths=No
     * ``softcap``: cap of the scores, 2^-10 to 2^10 (they are off by 2^-21 of it)
     * ``slopes`` fp32 [H]: linear bias by distance
 
+    Softmax statistics and sums are held in fp32; on the GPU the weights are rounded to q's type for the second product
+    (as in ``attention``).
     GPU: bf16 / fp16, D % 8 == 0, D <= 256 (csrc/masked_attention.hip).  Inference only."""
     qs, ks, dtype, device = q.shape, k.shape, q.dtype, q.device
     if len(qs) != 4 or len(ks) != 4 or ks != v.shape:

@@ -427,9 +427,9 @@ __device__ __forceinline__ void put_strip(const i32x16 (&acc)[TN][TM], int b, in
 // patch, so that a lane stores (and loads residuals) 8 channels wide with their scales in registers.
 // GLU: 32-row groups of the W tile alternate value rows and gate rows of the same channels, so both
 // halves of an output meet in one lane.
-// Bound by the matrix cores from 256 x 256 tiles on (16384 x 8192 x 8192: 937 us, 2346 Top/s; a library product of that
-// kind 2138), by LDS reads and the latency of a K step where a CU has one 64 x 128 tile (1232 x 4096 -> 1024: 14.4 us,
-// 717 Top/s).
+// Bound by the matrix cores from 256 x 256 tiles on (16384 x 8192 x 8192: 928 - 955 us, 2300 - 2370 Top/s; a library
+// product of that kind 2138), by LDS reads and the latency of a K step where a CU has one 64 x 128 tile
+// (1232 x 4096 -> 1024: 14.1 - 15 us, 690 - 730 Top/s).
 template <int EL, bool GLU, int BM, int BN, int WM, int WN, int NS>
 __global__ void __launch_bounds__(64 * WM * WN, 1) linear_int8_kernel(LinArgs p) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
@@ -739,8 +739,9 @@ __global__ void __launch_bounds__(64 * KW, 2) linear_int8_direct_kernel(LinArgs 
 // registers while the workgroup walks its weight rows, 64 at a time (GLU: 32 values and their 32 gates), through two
 // LDS stages.  A token's scale is a register of its lanes, so the epilogue runs in the accumulators' layout and only
 // the finished 16-bit channels cross lanes (LDS patch) for 16-byte stores.
-// Bound by the VALU (quantisation, scales, GELU) next to the write of y: LayerNorm 65536 x 320 -> 960 in 49.9 us (3.4
-// TB/s of x and y; apart 69.1), 16384 x 640 -> 5120 geglu in 87.7 us (1.2 Pop/s; apart 105.7).
+// Bound by the VALU (quantisation, scales, GELU) next to the write of y: LayerNorm 65536 x 320 -> 960 in 48 - 49
+// us with x and y's memory in the 256 MB cache (3.5 TB/s of them; quantised apart 69), 57 with x from memory, 61 - 68
+// with new memory for y too; 16384 x 640 -> 5120 geglu in 84 - 86 us launch behind launch, 91 - 94 alone (apart 106).
 template <int EL, bool GLU, bool LN, int KS, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) linear_int8_rows_kernel(LinArgs p, const uint16_t* __restrict__ x16,
                                                                       long ldx16, const uint16_t* __restrict__ gamma,

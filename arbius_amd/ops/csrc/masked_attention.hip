@@ -13,13 +13,14 @@ static KeyPlan key_plan(long batch, int H, int Hkv, int Nq, int Nk, int D) {
   const long rows = (long)(H / Hkv) * Nq, wgs = (rows + 127) / 128 * Hkv * batch;
   // Key ranges (a second kernel joins them): up to two workgroups per CU, 128 keys each at least, and not where
   // the partial sums written and read (8 D bytes a row and range) pass the keys and values read (4 D a key).  Measured,
-  // us: one token x 4, 65536 keys, 16 ranges 204, 8 ranges 265; 16 tokens, 8192 keys, 64 ranges 24, 8 ranges 40; one
-  // token x 16, 4096 keys, 4 ranges 54, 8 ranges 59.
+  // us, 32 heads on 8: one token x 4, 65536 keys, 16 ranges 193, 8 ranges 229; one token x 16, 4096 keys, 4 ranges 60,
+  // 8 ranges 61, 2 ranges 70; 16 heads on 4: 16 tokens, 8192 keys, 64 ranges 24, 8 ranges 29.
   long s = (512 + wgs - 1) / wgs;
   s = min(min(s, (Nk + 127L) / 128), min(256L, Nk / (2 * rows)));
   s = max(s, 1L);
-  // 8 waves where a CU gets one workgroup and the chain of tiles is long (us, against 4: 4096 tokens x 8 heads x 128
-  // 80.6 / 85.9, 8 x 2048 x 16 x 64 129 / 137); with more workgroups a second one is the second wave
+  // 8 waves where a CU gets one workgroup and the keys are many (causal, us, against 4: 4096 tokens x 8 heads x 128
+  // 69 / 87, 2 x 2047 x 8 x 80 36 / 41, 8192 x 4 x 64 82 / 105); with more workgroups a second one is the second wave
+  // (8 x 2048 x 16 x 64 144 / 114)
   const int wk = wgs * s <= 256 && Nk >= 512 && rows > 32 && D <= 128 ? 2 : 1;
   return {(int)s, wk};
 }

@@ -301,8 +301,8 @@ LARGE = {"256 x 256": (4100, 1101, 4099, 4098), "two stages": (2100, 1500, 2050,
                                                ("quick_gelu", False, "odd"), ("geglu", True, None)])
 @pytest.mark.parametrize("name", LARGE)
 def test_every_kernel_of_large_products(cuda, dtype, act, bias, residual, name):
-    """Widths that are no multiple of a vector, rows that are none of 16 bytes, residuals at odd elements: the element-wise
-    epilogue of every tile kernel; the same with a width of whole vectors."""
+    """Widths that are no multiple of a vector, rows that are none of 16 bytes, residuals at odd elements: the
+    element-wise epilogue of every tile kernel; the same with a width of whole vectors."""
     dt, (m, k, odd, glu) = DTYPES[dtype], LARGE[name]
     tiles = lambda bm, bn, n: -(-m // bm) * -(-n // bn)     # noqa: E731
     for n in ((glu if act == "geglu" else odd), (glu if act == "geglu" else odd) // 16 * 16):
@@ -585,8 +585,8 @@ def test_layernorm_batch_invariance(device, k):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("k", [8, 312, 320, 328, 640, 1000, 1280, 2048, 2560, 4096, 8192, 16384, 16392, 1001])
 def test_layernorm_order_is_the_lengths_alone(device, dtype, k):
-    """The same rows at an odd base, with a row stride that is no multiple of a vector, or alone, behind gamma and beta at
-    odd bases: the same 8 bits, scales and products."""
+    """The same rows at an odd base, with a row stride that is no multiple of a vector, or alone, behind gamma and
+    beta at odd bases: the same 8 bits, scales and products."""
     dt, m = DTYPES[dtype], 200 if k < 4000 else 40
     x = (randn(m, k, seed=1) * 3 + 0.5).to(dt).to(device)
     gamma, beta = (1 + 0.1 * randn(k, seed=2)).to(dt).to(device), (0.1 * randn(k, seed=3)).to(dt).to(device)

@@ -240,12 +240,14 @@ def test_a_value_reaches_only_the_queries_that_see_it(device, val):
         assert bool(got.isnan().all()) if math.isnan(val) else bool((got == val).all())
 
 
-SEEN = {   # values that are seen at a weight too small for 32 bits: parts of a split cache, the two-wave plan, one tile run
+# values that are seen at a weight too small for 32 bits: parts of a split cache, the two-wave plan, one run of tiles
+SEEN = {
     "split cache": dict(shape=(1, 1, 6000, 1, 1, 64), slopes=torch.tensor([0.5])),
     "split cache, heads": dict(shape=(2, 2, 5000, 4, 2, 128), causal=True, q_start=4000,
                                slopes=torch.tensor([0.5, 1.0, 2.0, 0.25])),
     "two waves on the keys": dict(shape=(1, 700, 700, 1, 1, 64), slopes=torch.tensor([2.0])),
-    "one wave, late maximum": dict(shape=(1, 40, 400, 8, 1, 80), causal=True, q_start=360, slopes=torch.full((8,), 2.0)),
+    "one wave, late maximum": dict(shape=(1, 40, 400, 8, 1, 80), causal=True, q_start=360,
+                                   slopes=torch.full((8,), 2.0)),
     "head 256": dict(shape=(1, 3, 900, 1, 1, 256), q_start=890, slopes=torch.tensor([1.0])),
 }
 
@@ -276,7 +278,8 @@ def test_a_seen_value_shows_at_any_weight(device, dtype, name):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("nq,nk,heads,start", [(140, 140, 2, 0), (1, 6000, 2, 5990), (700, 700, 1, 0), (2, 300, 4, 290)])
+@pytest.mark.parametrize("nq,nk,heads,start",
+                         [(140, 140, 2, 0), (1, 6000, 2, 5990), (700, 700, 1, 0), (2, 300, 4, 290)])
 def test_scores_that_are_all_minus_infinity(device, dtype, nq, nk, heads, start):
     """Keys, but none with a score above -inf: 0 / 0, where no keys give zeros; one finite score is enough for a row."""
     dt = DTYPES[dtype]
@@ -362,8 +365,8 @@ def test_strides_of_single_sizes(device):
             return store.as_strided((b, n, heads, 64), (*strides, 1), at)
         q, k, v = odd(nq, h, 0), odd(nk, hkv, 2048), odd(nk, hkv, 4096)
         got = ops.masked_attention(q, k, v, causal=True)
-        assert torch.equal(got, ops.masked_attention(*(t.clone(memory_format=torch.contiguous_format) for t in (q, k, v)),
-                                                     causal=True))
+        dense = (t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+        assert torch.equal(got, ops.masked_attention(*dense, causal=True))
     pair = i32([[2, 7], [1, 7]]).to(device)
     got = ops.masked_attention(*(t[:1] for t in (q, k, v)), causal=True, lengths=pair[1:, 0], q_start=pair[:1, 0],
                                prefix=pair[:1, 0])
@@ -609,8 +612,8 @@ def test_prompts_without_any_token(device, int8):
 @pytest.mark.gpu
 @pytest.mark.parametrize("int8", [False, True])
 def test_packed_prompts_in_a_graph(cuda, int8):
-    """One graph over ids and offsets that change between replays, with eager work in between: other prompts, empty ones,
-    one too long, and the same again."""
+    """One graph over ids and offsets that change between replays, with eager work in between: other prompts, empty
+    ones, one too long, and the same again."""
     from arbius_amd.models.graphs import GraphedCall
     clip = layers.init_weights(CLIPTextEncoder(CLIPTextConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256)), 1)
     xlmr = layers.init_weights(MCLIPText(XLMRConfig(vocab=1000, width=128, layers=2, heads=2, mlp=256, max_pos=100,
@@ -620,7 +623,8 @@ def test_packed_prompts_in_a_graph(cuda, int8):
         model.to(device=cuda, dtype=torch.bfloat16).eval()
         if int8:
             layers.int8_linears(model)
-        ids = [torch.randint(3, 900, (200,), generator=torch.Generator().manual_seed(s)).to(cuda) for s in (1, 2, 3, 4, 1)]
+        ids = [torch.randint(3, 900, (200,), generator=torch.Generator().manual_seed(s)).to(cuda)
+               for s in (1, 2, 3, 4, 1)]
         with torch.no_grad():
             want = [tuple(t.clone() for t in model.forward_packed(i, i32(off).to(cuda))) for i, off in zip(ids, packs)]
             graph = GraphedCall(model.forward_packed, [ids[0], i32(packs[0]).to(cuda)])
