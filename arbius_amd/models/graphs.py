@@ -109,8 +109,8 @@ def live_table(tensors) -> list:
 
 
 def stale(graph) -> bool:
-    """Whether layers of a captured graph (its ``uses``) have changed between 16 and 8 bits since; waits for its replays
-    then, so that the caller can drop it and capture again."""
+    """Whether layers of a captured graph (its ``uses``) have changed between 16 and 8 bits, or in 8 bits, since; waits
+    for its replays then, so that the caller can drop it and capture again."""
     if graph.uses.current():
         return False
     with CAPTURE_LOCK:
@@ -123,7 +123,7 @@ def check_live(table, uses) -> None:
     storage size), every captured layer in the form it had.  A replay into a moved or re-sized block would write
     another tensor's memory."""
     if not uses.current():
-        raise RuntimeError("graph captured with layers that have changed between 16 and 8 bits since")
+        raise RuntimeError("graph captured with layers that have changed between 16 and 8 bits, or in 8 bits, since")
     for t, ptr, nbytes in table:
         if t.data_ptr() != ptr or t.untyped_storage().nbytes() != nbytes:
             raise RuntimeError(f"graph buffer moved: {ptr:#x} -> {t.data_ptr():#x} "
@@ -171,7 +171,7 @@ class GraphedCall:
 
 class GraphCache:
     """Graphs keyed by input shapes (one per resolution / batch); captured again where layers have changed between 16
-    and 8 bits (``layers.int8_linears``)."""
+    and 8 bits (``layers.int8_linears``), or the weights of 8-bit ones."""
 
     def __init__(self, fn: Callable, enabled: bool):
         self.fn, self.enabled = fn, enabled

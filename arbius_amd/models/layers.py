@@ -29,10 +29,10 @@ _SWITCHES = [None]               # another object after every change of a layer 
 class Int8Uses:
     """``with Int8Uses() as uses:`` - the form (``Int8Rows``, or None: 16 bits) of every ``Linear`` that this thread
     runs meanwhile.  A captured graph keeps one: it holds the 8-bit tensors whose addresses the graph replays, and
-    ``current`` tells whether the layers still have the form that was captured."""
+    ``current`` tells whether they still are what the layers would run on."""
 
     def __init__(self):
-        self.forms, self.seen = {}, _SWITCHES[0]
+        self.forms, self.weights, self.seen = {}, (), _SWITCHES[0]
 
     def __enter__(self):
         self.prev, _USES.log = getattr(_USES, "log", None), self.forms
@@ -40,6 +40,8 @@ class Int8Uses:
 
     def __exit__(self, *exc):
         _USES.log = self.prev
+        self.weights = [(lin._parameters, lin._parameters["weight"], *lin._of[:2])
+                        for lin, form in self.forms.values() if form is not None and form is lin.int8]
 
     def current(self) -> bool:
         switches = _SWITCHES[0]
@@ -47,6 +49,9 @@ class Int8Uses:
             if any(lin.int8 is not form for lin, form in self.forms.values()):
                 return False
             self.seen = switches
+        for params, w, ptr, version in self.weights:               # as Linear.outdated, before every replay
+            if w._version != version or w.data_ptr() != ptr or params["weight"] is not w:
+                return False
         return True
 
 
@@ -80,13 +85,18 @@ class Linear(nn.Module):
         if self.bias is not None:
             self.bias.data.uniform_(-bound, bound, generator=gen)
 
+    def outdated(self) -> bool:
+        """Whether the weight holds other values than its 8-bit form was made of."""
+        return self._of != self._weight()
+
     def form(self):
         """The ``Int8Rows`` this layer runs on, None in 16 bits; noted for the capture under way on this thread."""
         int8, log = self._int8, getattr(_USES, "log", None)
-        if int8 is not None and self._of != self._weight():        # other values than were quantised
-            int8 = ops.quantize_rows(self.weight)
-            ops.derived_ready(int8.q)
-            self.int8 = int8
+        if int8 is not None and self.outdated():
+            with CAPTURE_LOCK:                                     # forks come here at once: one of them quantises
+                if self.outdated():
+                    _publish([self], [ops.quantize_rows(self.weight)])
+                int8 = self._int8
         if log is not None:
             log[id(self), id(int8)] = self, int8
         return int8
@@ -226,16 +236,22 @@ def int8_linears(module: nn.Module, on: bool = True) -> int:
     """Run the ``Linear`` layers of ``module`` in 8 bits (``ops.linear_int8``; weights quantised here, once, per output
     channel; activations per token as they come) or, with ``on=False``, in their own type again.  An
     operator's choice per deployment: other bytes than the 16-bit layers, so never for a registered model
-    whose solutions other nodes verify.  Returns the number of layers.  Weights loaded or moved later are
-    quantised again at their next use (changed through ``.data``, which torch does not count, only by another call);
-    ``hoisted`` layers, of which only the bare weight is used, stay in 16 bits and are not counted.
+    whose solutions other nodes verify.  Returns the number of layers; ``hoisted`` ones, of which only the bare
+    weight is used, stay in 16 bits and are not counted.  Weights loaded or moved later are quantised again at their
+    next use (changed through ``.data``, which torch does not count, only by another call).
 
     All weights are quantised before the first layer changes, and their kernels have finished: pipeline forks share
-    the layers across threads and streams (``ops.derived_ready``).  Pipelines capture their graphs again at the next
-    call.  Call it while none is solving: 8-bit weights that it replaces are given back once what the GPUs were
-    doing is done."""
+    the layers across threads and streams (``ops.derived_ready``).  Pipelines capture their graphs again at their next
+    call, after this one and after a change of weights.  Call it while none is solving: 8-bit weights that it replaces
+    are given back once what the GPUs were doing is done."""
     linears = [m for m in module.modules() if isinstance(m, Linear) and not m.hoisted]
-    forms = [ops.quantize_rows(m.weight) if on else None for m in linears]
+    _publish(linears, [ops.quantize_rows(m.weight) if on else None for m in linears])
+    return len(linears)
+
+
+def _publish(linears, forms):
+    """Give the layers these 8-bit forms (or None) once the kernels that write them have finished, and give the old ones
+    back once the kernels of any stream that read them have."""
     for q in {f.device: f.q for f in forms if f is not None}.values():
         ops.derived_ready(q)
     old = {}
@@ -243,11 +259,10 @@ def int8_linears(module: nn.Module, on: bool = True) -> int:
         if m.int8 is not None:
             old.setdefault(m.int8.device, []).append(m.int8)
         m.int8 = form
-    for device in old:                 # read by kernels of any stream so far
+    for device in old:
         if device.type == "cuda":
             with CAPTURE_LOCK:         # a device is not waited for while a thread captures on it
                 torch.cuda.synchronize(device)
-    return len(linears)
 
 
 def timestep_embedding(t, dim, flip_sin_to_cos=True, freq_shift=0.0, max_period=10000):

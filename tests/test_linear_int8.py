@@ -453,6 +453,14 @@ def test_a_capture_knows_the_forms_it_used():
     assert not b.current() and not a.current()
     m.fc2.int8 = None
     assert a.current() and not b.current()
+    layers.int8_linears(m)
+    c = capture()
+    assert c.current()
+    m.load_state_dict(other.state_dict())                    # other weights
+    assert not c.current()
+    d = capture()
+    assert d.current() and not c.current()
+    layers.int8_linears(m, False)
     m(x)                                                     # outside of a capture nothing is noted
     assert len(a.forms) == 2
 
@@ -490,6 +498,33 @@ def test_captured_graphs_follow_the_layers(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("graphs", [False, True])
+def test_forks_in_8_bits_at_once(cuda, graphs):
+    """Two forks on their own threads and streams whose first use of changed weights comes at once: what each answers
+    alone afterwards."""
+    from concurrent.futures import ThreadPoolExecutor
+    from arbius_amd.models.registry import build_pipeline
+    pipe = build_pipeline("anythingv3", device=cuda, use_graphs=graphs)
+    for m in (pipe.unet, pipe.text):
+        layers.int8_linears(m)
+    kws = [dict(prompt=f"a lake {i}", width=128, height=128, num_inference_steps=2, scheduler="DPMSolverMultistep",
+                seed=i) for i in range(2)]
+    forks, last = [pipe.fork() for _ in kws], None
+    for _ in range(3):
+        with torch.no_grad():
+            for m in (*pipe.text.modules(), *pipe.unet.modules()):
+                if isinstance(m, layers.Linear):
+                    m.weight.mul_(1.0625)
+        torch.cuda.synchronize()
+        with ThreadPoolExecutor(2) as ex:
+            got = list(ex.map(lambda a: a[0](**a[1]), zip(forks, kws)))
+        want = [pipe(**kw) for kw in kws]
+        assert all((g == w).all() for g, w in zip(got, want))
+        assert last is None or (last != want[0]).any()
+        last = want[0]
+
+
+@pytest.mark.gpu
 def test_a_graph_of_other_forms_is_refused(cuda):
     from arbius_amd.models.graphs import GraphCache, GraphedCall
     m = layers.init_weights(_Block(), 3).to(device=cuda, dtype=torch.bfloat16)
@@ -504,6 +539,14 @@ def test_a_graph_of_other_forms_is_refused(cuda):
     assert torch.equal(cache(x), want8) and not torch.equal(want, want8)
     layers.int8_linears(m, False)
     assert torch.equal(cache(x), want) and torch.equal(old(x), want)
+    layers.int8_linears(m)
+    old = GraphedCall(m, [x])
+    assert torch.equal(cache(x), want8) and torch.equal(old(x), want8)
+    m.load_state_dict(layers.init_weights(_Block(), 5).state_dict())
+    with pytest.raises(RuntimeError, match="8 bits"):
+        old(x)
+    got = cache(x).clone()
+    assert torch.equal(got, m(x)) and not torch.equal(got, want8)
 
 
 @pytest.mark.gpu
